@@ -92,6 +92,15 @@ _SIGS = {
     'ag2v_col_sum': (c_int, [_P, _P, c_int, c_int, _P]),
     'ag2v_embedding_fwd': (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     'ag2v_embedding_bwd': (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
+    'ag2v_embed_fwd': (c_int, [c_int, _P, c_int, c_longlong, _P, c_longlong, _P, c_longlong, c_longlong, c_int, c_float, _P]),
+    'ag2v_embed_bwd_workspace_floats': (c_size_t, [c_int, c_longlong, c_longlong, c_int]),
+    'ag2v_embed_bwd': (c_int, [c_int, _P, c_int, c_longlong, _P, c_longlong, _P, c_longlong, c_longlong, c_int, c_float, c_longlong, _P,
+                               c_size_t, _P]),
+    'ag2v_group_norm_workspace_floats': (c_size_t, [c_int] * 6),
+    'ag2v_group_norm_fwd': (c_int, [c_int, _P, c_longlong, c_longlong, _P, _P, c_int, _P, _P, _P] + [c_int] * 4 +
+                            [c_float, c_int, c_float, _P, c_size_t, _P]),
+    'ag2v_group_norm_bwd': (c_int, [c_int, _P, c_longlong, c_longlong, _P, c_longlong, c_longlong, _P, _P, c_int] + [_P] * 5 +
+                            [c_int] * 5 + [c_float, _P, c_size_t, _P]),
     'ag2v_act_fwd': (c_int, [c_int, _P, _P, c_longlong, c_float, _P]),
     'ag2v_act_bwd': (c_int, [c_int, _P, _P, _P, c_longlong, c_float, _P]),
     'ag2v_reduce_workspace_floats': (c_size_t, []),

@@ -17,8 +17,28 @@ class Linear(nn.Linear):
 
 
 class Embedding(nn.Embedding):
+    """``scale`` (a number), ``padding_idx`` or a 16-bit table: ops.embedding_scaled (gradient by sorted tokens: for large vocabularies and
+    long inputs).  Neither, in fp32: ops.embedding, as every table of the models here."""
+
+    def __init__(self, *args, scale=None, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.scale = scale
+
     def forward(self, idx):
-        return ops.embedding(idx, self.weight)
+        if self.scale is None and self.padding_idx is None and self.weight.dtype == torch.float32:
+            return ops.embedding(idx, self.weight)
+        return ops.embedding_scaled(idx, self.weight, 1.0 if self.scale is None else self.scale, self.padding_idx)
+
+
+class GroupNormAct(nn.GroupNorm):
+    """Group norm with the activation behind it, on channels-last maps [N, ..., C] (nn.GroupNorm's parameters and state_dict names)."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, act='silu', slope=0.2, device=None, dtype=None):
+        super().__init__(num_groups, num_channels, eps=eps, affine=affine, device=device, dtype=dtype)
+        self.act, self.slope = act, slope
+
+    def forward(self, x):
+        return ops.group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act, self.slope)
 
 
 class Conv2d(nn.Conv2d):

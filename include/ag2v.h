@@ -365,6 +365,39 @@ int ag2v_embedding_fwd(const long long* idx, const float* table, float* out, int
 int ag2v_embedding_bwd(const long long* idx, const float* dout, float* dtable, int n, int V, int D, int in_stride, int in_off,
                        void* stream);
 
+/* ---- fp32 / bf16 / fp16 operators ------------------------------------------------------------------------------------
+ * `dtype` / `param_dtype`: the element type of the tensors a call names as void*.  Sums and products are in fp32 (a few joins in fp64)
+ * and rounded once, to nearest even.  Rows may start at any multiple of the element's size. */
+#define AG2V_F32 0
+#define AG2V_BF16 1
+#define AG2V_F16 2
+
+/* Embedding lookup with scaling: out[i,:] = scale * table[idx_i,:] (out contiguous [n,D]); the rows of `table` are table_stride elements
+ * apart, the tokens idx (int32 or int64: idx_bytes 4 / 8) idx_stride elements.  A token outside [0,V) reads nothing and gives a row of NaN.
+ * Gradient: dtable[v,:] = scale * (sum of the rows dout[i,:] with idx_i = v), written densely ([V,D], contiguous; rows no token names and the
+ * row padding_idx are zero; padding_idx < 0: none).  The tokens are sorted (stably) and the rows summed in ascending order inside ranges
+ * that the sizes alone fix: no atomics, equal calls give equal bits.  dout_stride may be 0 (one row for all).  n, V < 2^31.
+ * workspace: ag2v_embed_bwd_workspace_floats() floats. */
+int ag2v_embed_fwd(int dtype, const void* idx, int idx_bytes, long long idx_stride, const void* table, long long table_stride, void* out,
+                   long long n, long long V, int D, float scale, void* stream);
+size_t ag2v_embed_bwd_workspace_floats(int dtype, long long n, long long V, int D);
+int ag2v_embed_bwd(int dtype, const void* idx, int idx_bytes, long long idx_stride, const void* dout, long long dout_stride, void* dtable,
+                   long long n, long long V, int D, float scale, long long padding_idx, float* workspace, size_t workspace_floats,
+                   void* stream);
+
+/* Group norm with an activation, channels last: x[N,S,C] (strides x_sample / x_row in elements, channels adjacent), y contiguous,
+ * weight / bias [C] of param_dtype or NULL (1 / 0), mean / rstd fp32 [N,groups] written for the backward pass.
+ * act: 0 none, 1 silu, 2 leaky relu of `slope`.  Backward: dx (contiguous), dweight, dbias (param_dtype); each may be NULL.
+ * No atomics: equal calls give equal bits.  workspace: ag2v_group_norm_workspace_floats(..., backward) floats. */
+size_t ag2v_group_norm_workspace_floats(int dtype, int N, int S, int C, int groups, int backward);
+int ag2v_group_norm_fwd(int dtype, const void* x, long long x_sample, long long x_row, const void* weight, const void* bias, int param_dtype,
+                        void* y, float* mean, float* rstd, int N, int S, int C, int groups, float eps, int act, float slope,
+                        float* workspace, size_t workspace_floats, void* stream);
+int ag2v_group_norm_bwd(int dtype, const void* dy, long long dy_sample, long long dy_row, const void* x, long long x_sample, long long x_row,
+                        const void* weight, const void* bias, int param_dtype, const float* mean, const float* rstd, void* dx, void* dweight,
+                        void* dbias, int N, int S, int C, int groups, int act, float slope, float* workspace, size_t workspace_floats,
+                        void* stream);
+
 /* ---- pointwise + losses: F.leaky_relu / tanh (spade_generator.py:78-80); GANLoss hinge networks/loss.py:57-76;
  * L1 feature matching / flow-warp loss_model.py:84,97 ------------------------------------------------------------- */
 int ag2v_act_fwd(int op /*0 lrelu, 1 tanh*/, const float* x, float* y, long long n, float slope, void* stream);

@@ -1,0 +1,513 @@
+"""embedding_scaled and group_norm_act against 64-bit references with derived bounds (tests/_elem_ref.py)."""
+import pytest
+import torch
+
+import _elem_ref as R
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ['f32', 'bf16', 'f16']
+
+
+def _randn(*shape, seed, scale=1.0, shift=0.0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale + shift).to(dtype)
+
+
+def _tokens(n, V, seed, kind='uniform'):
+    g = torch.Generator().manual_seed(seed)
+    if kind == 'uniform':
+        return torch.randint(V, (n,), generator=g)
+    if kind == 'one':                                      # every token the same: one long segment
+        return torch.full((n,), V // 2)
+    if kind == 'skewed':                                   # half of all tokens are one word, the rest follow 1 / rank
+        t = (torch.exp(torch.rand(n, generator=g, dtype=torch.float64) * torch.log(torch.tensor(V + 1.0, dtype=torch.float64))) - 1).long().clamp(0, V - 1)
+        return torch.where(torch.rand(n, generator=g) < 0.5, torch.full_like(t, V - 1), t)
+    if kind == 'sorted':
+        return torch.randint(V, (n,), generator=g).sort().values
+    return torch.arange(n) % V                             # 'cyclic'
+
+
+def _embed_case(device, idx, table, scale, pad, dout, name):
+    from ag2video_amd import ops
+    ref = R.embedding(idx, table, scale, pad, dout)
+    t = table.to(device).requires_grad_(True)
+    i = idx.to(device)
+    out = ops.embedding_scaled(i, t, scale, pad)
+    assert out.dtype == table.dtype and out.device == t.device
+    R.check(name + '.out', out, ref[0], ref[1])
+    (dt,) = torch.autograd.grad(out, t, dout.to(device))
+    assert dt.dtype == table.dtype
+    R.check(name + '.dtable', dt, ref[2], ref[3])
+    with torch.no_grad():                                  # the path without a tape, and a second call: the same bits
+        assert torch.equal(ops.embedding_scaled(i, t, scale, pad).nan_to_num(7.0), out.detach().nan_to_num(7.0))
+    (again,) = torch.autograd.grad(ops.embedding_scaled(i, t, scale, pad), t, dout.to(device))
+    assert torch.equal(dt, again)
+
+
+EMBED = [
+    # n, V, D, tokens
+    (1, 1, 1, 'uniform'), (1, 5, 3, 'uniform'), (2, 1, 8, 'uniform'), (7, 3, 7, 'cyclic'), (10, 24, 128, 'uniform'),
+    (63, 64, 16, 'cyclic'), (64, 64, 16, 'cyclic'), (65, 1000, 9, 'sorted'), (257, 2, 33, 'uniform'), (1280, 24, 128, 'uniform'),
+    (1000, 7, 520, 'one'), (300, 40000, 12, 'uniform'), (4095, 511, 40, 'skewed'), (4096, 512, 24, 'sorted'), (4097, 513, 17, 'skewed'),
+    (3, 70001, 2, 'uniform'), (2000, 100, 1027, 'skewed'),
+    (8191, 33000, 31, 'skewed'), (8192, 300, 64, 'one'), (8193, 70000, 5, 'uniform'),
+    (20000, 1025, 16, 'skewed'), (20001, 3, 48, 'uniform'), (33333, 60, 129, 'sorted'), (70000, 1, 4, 'one'), (66000, 262145, 4, 'uniform'),
+    (120000, 5000, 1, 'skewed'),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("n,V,D,kind", EMBED, ids=lambda v: str(v))
+def test_embedding_scaled(n, V, D, kind, dtype, device):
+    idx = _tokens(n, V, n + V, kind)
+    _embed_case(device, idx, _randn(V, D, seed=1, dtype=dtype), 0.37, None, _randn(n, D, seed=2, scale=0.1, dtype=dtype), 'embed')
+
+
+@pytest.mark.parametrize("pad", [None, 0, 11], ids=str)
+@pytest.mark.parametrize("shape", [(), (5,), (3, 4), (2, 3, 50), (0,), (4, 0)], ids=str)
+def test_embedding_scaled_shapes_and_padding(shape, pad, device):
+    n = 1
+    for s in shape:
+        n *= s
+    for itype in (torch.int32, torch.int64):
+        idx = _tokens(n, 12, 5).view(shape).to(itype)
+        _embed_case(device, idx, _randn(12, 20, seed=1), 4.5, pad, _randn(*shape, 20, seed=2), 'embed')
+
+
+@pytest.mark.parametrize("n,V", [(40, 30), (3000, 30), (3000, 30000), (40000, 30)], ids=str)
+def test_embedding_scaled_foreign_tokens(n, V, device):
+    """Tokens outside the table: a row of NaN, no part in any gradient, nothing else disturbed."""
+    idx = _tokens(n, V, 3)
+    idx[::7] = V
+    idx[1::11] = -1
+    idx[2::13] = 2 ** 40
+    idx[3::17] = -2 ** 62
+    _embed_case(device, idx, _randn(V, 24, seed=1), 1.0, 2, _randn(n, 24, seed=2), 'foreign')
+    idx = torch.full((n,), V)
+    _embed_case(device, idx, _randn(V, 24, seed=1), 1.0, None, _randn(n, 24, seed=2), 'all foreign')
+
+
+def test_embedding_scaled_strides(device):
+    """Token and gradient views, a table inside a wider one and at an odd offset."""
+    from ag2video_amd import ops
+    base = _tokens(6 * 7 * 3, 9, 1).view(6, 7, 3)
+    wide = _randn(9, 40, seed=2)
+    for name, pick in (('slice', lambda t: t[:, :, 1]), ('transposed', lambda t: t.permute(2, 0, 1)), ('every other', lambda t: t[::2]),
+                       ('expanded', lambda t: t[:1].expand(5, 7, 3)), ('reversed order', lambda t: t.transpose(0, 1))):
+        idx = pick(base)
+        table = wide[:, 3:24]
+        dout = _randn(*idx.shape, 21, seed=3)
+        out_ref, b_out, dt_ref, b_dt = R.embedding(idx, table, 1.5, None, dout)
+        leaf = wide.to(device).requires_grad_(True)
+        out = ops.embedding_scaled(pick(base.to(device)), leaf[:, 3:24], 1.5)
+        R.check(name + '.out', out, out_ref, b_out)
+        (g,) = torch.autograd.grad(out, leaf, dout.to(device))
+        R.check(name + '.dtable', g[:, 3:24], dt_ref, b_dt)
+        assert not g[:, :3].any() and not g[:, 24:].any()
+    # broadcast gradients (sum().backward()) and gradients whose rows lie apart
+    idx, table = base[..., 0].contiguous(), wide.to(device).requires_grad_(True)
+    for name, d in (('ones', torch.ones(()).expand(6, 7, 40)), ('one row', _randn(40, seed=4).expand(6, 7, 40)),
+                    ('row stride', _randn(6, 7, 50, seed=5)[..., 5:45]), ('transposed', _randn(40, 6, 7, seed=6).permute(1, 2, 0))):
+        ref = R.embedding(idx, wide, 2.0, None, d)
+        (g,) = torch.autograd.grad(ops.embedding_scaled(idx.to(device), table, 2.0), table, d.to(device))
+        R.check(name, g, ref[2], ref[3])
+    flat = _randn(9 * 13 + 1, seed=7, dtype=torch.bfloat16).to(device)         # rows at 2-byte offsets
+    table = flat[1:].view(9, 13)
+    ref = R.embedding(idx, table.cpu(), 1.0, None)
+    R.check('offset', ops.embedding_scaled(idx.to(device), table), *ref)
+
+
+def test_embedding_scaled_special_values(device):
+    """Infinities and NaN stay in the rows and columns they are in."""
+    V, D, n = 6, 10, 50
+    table, dout, idx = _randn(V, D, seed=1), _randn(n, D, seed=2), _tokens(n, V, 3)
+    table[2, 3], table[4, 0] = float('inf'), float('nan')
+    from ag2video_amd import ops
+    out = ops.embedding_scaled(idx.to(device), table.to(device), 2.0).cpu()
+    assert torch.equal(out.nan_to_num(5.0, 6.0, 7.0), (table[idx] * 2.0).nan_to_num(5.0, 6.0, 7.0))
+    i2, i3 = int((idx == 2).nonzero()[0]), int((idx == 3).nonzero()[0])
+    dout[i2, 1], dout[i3, 2] = float('nan'), float('-inf')
+    leaf = _randn(V, D, seed=1).to(device).requires_grad_(True)
+    (g,) = torch.autograd.grad(ops.embedding_scaled(idx.to(device), leaf, 2.0, 5), leaf, dout.to(device))
+    g = g.cpu()
+    assert torch.isnan(g[2, 1]) and g[3, 2] == float('-inf') and int((~torch.isfinite(g)).sum()) == 2
+    assert not g[5].any()
+
+
+def test_embedding_scaled_long_offsets(device):
+    """Offsets of the output beyond 2^31 elements and 2^32 bytes."""
+    from ag2video_amd import ops
+    n, D, V = (1 << 25) + 77, 72, 50                       # 2.4e9 elements
+    idx = (torch.arange(n, device=device) * 7) % V
+    table = _randn(V, D, seed=1, dtype=torch.bfloat16).to(device).requires_grad_(True)
+    out = ops.embedding_scaled(idx, table, 2.0)
+    for at in (0, 12345, (1 << 31) // D, (1 << 31) // D + 1, n - 1):
+        assert torch.equal(out[at], table.detach()[at * 7 % V] * 2.0)
+    dout = torch.zeros(1, device=device, dtype=torch.bfloat16).expand(n, D)
+    (g,) = torch.autograd.grad(out, table, dout)
+    assert not g.any()
+    del dout
+    # a gradient of ones counts the tokens; counts are sums of halves of 2^-1 exactly while they stay below 2^24 in fp32
+    ones = torch.ones(n, 4, device=device).expand(n, 4)
+    small = torch.zeros(V, 4, device=device, requires_grad=True)
+    (g,) = torch.autograd.grad(ops.embedding_scaled(idx, small, 0.5), small, ones)
+    assert torch.equal(g, 0.5 * torch.bincount(idx, minlength=V).float()[:, None].expand(V, 4))
+
+
+NORM = [
+    # shape, groups
+    ((1, 1), 1), ((3, 4), 2), ((2, 1, 6), 6), ((1, 5, 7), 7), ((2, 9, 8), 1), ((3, 37, 90), 6), ((2, 16, 64), 4), ((1, 1000, 33), 3),
+    ((4, 64, 64), 32), ((1, 63, 512), 32), ((2, 129, 40), 5), ((1, 17, 2050), 1), ((1, 3, 4104), 2), ((2, 2048, 16), 2), ((2, 7, 5, 3, 24), 3),
+    ((200, 2, 24), 3), ((3000, 1, 8), 2), ((1, 1500, 6), 1), ((2, 700, 1030), 2), ((1, 1, 9000), 3), ((2, 40 * 40, 96), 32), ((1, 6000, 320), 32),
+    ((2, 5000, 3), 3), ((1, 20, 512), 512),
+]
+
+
+def _norm_case(device, shape, groups, dtype, act, affine, ptype, seed=1, eps=1e-5, slope=0.2, shift=1.0):
+    from ag2video_amd import ops
+    C = shape[-1]
+    x = (_randn(*shape, seed=seed) * torch.exp(0.3 * _randn(C, seed=seed + 1)) + shift * _randn(C, seed=seed + 2)).to(dtype)
+    w = (1 + 0.3 * _randn(C, seed=seed + 3)).to(ptype) if affine else None
+    b = _randn(C, seed=seed + 4, scale=0.3).to(ptype) if affine else None
+    dy = _randn(*shape, seed=seed + 5).to(dtype)
+    ref = R.group_norm(x, groups, w, b, eps, act, slope, dy)
+    leaves = [t.to(device).requires_grad_(True) for t in (x, w, b) if t is not None]
+    y = ops.group_norm_act(leaves[0], groups, *(leaves[1:] or (None, None)), eps=eps, act=act, slope=slope)
+    assert y.dtype == dtype and y.is_contiguous()
+    R.check('y', y, *ref['y'])
+    grads = torch.autograd.grad(y, leaves, dy.to(device))
+    for name, g, leaf in zip(('dx', 'dweight', 'dbias'), grads, leaves):
+        assert g.dtype == leaf.dtype
+        R.check(name, g, *ref[name])
+    with torch.no_grad():
+        y2 = ops.group_norm_act(leaves[0], groups, *(leaves[1:] or (None, None)), eps=eps, act=act, slope=slope)
+    assert torch.equal(y2, y.detach())
+    again = torch.autograd.grad(ops.group_norm_act(leaves[0], groups, *(leaves[1:] or (None, None)), eps=eps, act=act, slope=slope), leaves, dy.to(device))
+    assert all(torch.equal(p, q) for p, q in zip(grads, again))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("shape,groups", NORM, ids=str)
+def test_group_norm_act(shape, groups, dtype, device):
+    _norm_case(device, shape, groups, dtype, 'silu', True, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("act", ['none', 'silu', 'lrelu'])
+@pytest.mark.parametrize("affine", [False, True], ids=['plain', 'affine'])
+def test_group_norm_act_forms(act, affine, dtype, device):
+    for shape, groups in (((2, 50, 24), 3), ((2, 3000, 36), 4), ((2, 9, 10), 2)):
+        _norm_case(device, shape, groups, dtype, act, affine, dtype, seed=7)
+        _norm_case(device, shape, groups, dtype, act, affine, torch.float32, seed=9, eps=0.1, slope=0.0)
+
+
+def test_group_norm_act_far_mean(device):
+    """A mean 300 deviations away, and one value 1e4 deviations away at the start of a group: the variance does not cancel."""
+    from ag2video_amd import ops
+    for shape, groups in (((2, 64, 16), 2), ((2, 6000, 16), 2)):
+        x = _randn(*shape, seed=3) + 300.0
+        x[0, 0, 0] += 1e4
+        dy = _randn(*shape, seed=4)
+        ref = R.group_norm(x, groups, None, None, 1e-5, 'none', 0.2, dy)
+        leaf = x.to(device).requires_grad_(True)
+        y = ops.group_norm_act(leaf, groups, act='none')
+        R.check('y', y, *ref['y'])
+        R.check('dx', torch.autograd.grad(y, leaf, dy.to(device))[0], *ref['dx'])
+
+
+@pytest.mark.parametrize("S", [30, 5000])
+def test_group_norm_act_one_parameter(S, device):
+    """weight without bias, bias without weight; gradients of a part of the inputs."""
+    from ag2video_amd import ops
+    x, p, dy = _randn(2, S, 12, seed=1), _randn(12, seed=2), _randn(2, S, 12, seed=3)
+    for w, b in ((p, None), (None, p)):
+        ref = R.group_norm(x, 3, w, b, 1e-5, 'silu', 0.2, dy)
+        gp = p.to(device).requires_grad_(True)
+        gx = x.to(device).requires_grad_(True)
+        args = (gp if w is not None else None, gp if b is not None else None)
+        y = ops.group_norm_act(gx, 3, *args)
+        R.check('y', y, *ref['y'])
+        dx, dp = torch.autograd.grad(y, (gx, gp), dy.to(device))
+        R.check('dx', dx, *ref['dx'])
+        R.check('dp', dp, *ref['dweight' if w is not None else 'dbias'])
+        only_p = torch.autograd.grad(ops.group_norm_act(gx.detach(), 3, *args), gp, dy.to(device))[0]
+        assert torch.equal(only_p, dp)
+        only_x = torch.autograd.grad(ops.group_norm_act(gx, 3, *(None if a is None else a.detach() for a in args)), gx, dy.to(device))[0]
+        assert torch.equal(only_x, dx)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+def test_group_norm_act_strides(dtype, device):
+    """Channel slices, channels-last NCHW tensors, samples apart, channels first (copied); gradients that are broadcast or lie apart."""
+    from ag2video_amd import ops
+    w, b = _randn(20, seed=8).to(device), _randn(20, seed=9).to(device)
+    views = {
+        'channel slice': (lambda t: t[..., 5:25], (3, 11, 13, 33)), 'one position apart': (lambda t: t[:, :, ::2], (3, 11, 14, 20)),
+        'every other sample': (lambda t: t[::2], (5, 40, 20)), 'channels first': (lambda t: t.permute(0, 2, 3, 1), (2, 20, 9, 7)),
+        'transposed positions': (lambda t: t.transpose(1, 2), (2, 9, 31, 20)), 'one sample repeated': (lambda t: t.expand(4, 30, 20), (1, 30, 20)),
+        'odd offset': (lambda t: t.reshape(-1)[1:1 + 3 * 70 * 20].view(3, 70, 20), (3, 71, 20)),
+        'long rows': (lambda t: t[..., 2:22], (2, 4500, 23)),
+    }
+    for name, (view, shape) in views.items():
+        base = _randn(*shape, seed=1).to(dtype)
+        x = view(base)
+        dy = _randn(*x.shape, seed=2).to(dtype)
+        ref = R.group_norm(x, 5, w.cpu(), b.cpu(), 1e-5, 'silu', 0.2, dy)
+        leaf = base.to(device).requires_grad_(True)
+        dx_at = view(leaf)
+        dx_at.retain_grad()
+        y = ops.group_norm_act(dx_at, 5, w, b)
+        R.check(name + '.y', y, *ref['y'])
+        y.backward(dy.to(device))
+        R.check(name + '.dx', dx_at.grad, *ref['dx'])
+    nchw = _randn(2, 20, 9, 7, seed=3).to(device).to(memory_format=torch.channels_last)
+    ref = R.group_norm(nchw.cpu().permute(0, 2, 3, 1), 5, w.cpu(), b.cpu(), 1e-5, 'silu', 0.2)
+    R.check('channels_last', ops.group_norm_act(nchw.permute(0, 2, 3, 1), 5, w, b), *ref['y'])
+    x = _randn(2, 9, 7, 20, seed=4).to(dtype)
+    for name, d in (('ones', torch.ones((), dtype=dtype).expand(2, 9, 7, 20)), ('one row', _randn(20, seed=5).to(dtype).expand(2, 9, 7, 20)),
+                    ('slice', _randn(2, 9, 7, 30, seed=6).to(dtype)[..., 3:23]), ('channels first', _randn(2, 20, 9, 7, seed=7).to(dtype).permute(0, 2, 3, 1))):
+        ref = R.group_norm(x, 5, w.cpu(), b.cpu(), 1e-5, 'silu', 0.2, d)
+        leaf = x.to(device).requires_grad_(True)
+        R.check(name, torch.autograd.grad(ops.group_norm_act(leaf, 5, w, b), leaf, d.to(device))[0], *ref['dx'])
+
+
+@pytest.mark.parametrize("S", [20, 7000])
+def test_group_norm_act_special_values(S, device):
+    """An infinity or NaN reaches its own (sample, group) only; other groups keep their bits, forward and backward."""
+    from ag2video_amd import ops
+    x, dy, w, b = _randn(3, S, 16, seed=1), _randn(3, S, 16, seed=2), _randn(16, seed=3).to(device), _randn(16, seed=4).to(device)
+
+    def run(x, dy):
+        leaf = x.to(device).requires_grad_(True)
+        y = ops.group_norm_act(leaf, 4, w, b)
+        return y.detach().cpu(), torch.autograd.grad(y, leaf, dy.to(device))[0].cpu()
+
+    y0, d0 = run(x, dy)
+    x[1, S // 2, 5], x[2, 0, 15] = float('inf'), float('nan')
+    y1, d1 = run(x, dy)
+    bad = torch.zeros(3, S, 16, dtype=torch.bool)
+    bad[1, :, 4:8] = bad[2, :, 12:16] = True
+    for p, q in ((y0, y1), (d0, d1)):
+        assert torch.isnan(q[bad]).all() and torch.equal(p[~bad], q[~bad])
+    x[1, S // 2, 5], x[2, 0, 15] = 0.0, 0.0
+    y2, d2 = run(x, dy)
+    dy[0, 3, 1] = float('nan')
+    y3, d3 = run(x, dy)
+    bad = torch.zeros(3, S, 16, dtype=torch.bool)
+    bad[0, :, :4] = True
+    assert torch.equal(y2, y3) and torch.isnan(d3[bad]).all() and torch.equal(d2[~bad], d3[~bad])
+
+
+def test_group_norm_act_constant_groups(device):
+    """Variance zero: h = 0, y = act(bias), and a gradient that stays finite."""
+    from ag2video_amd import ops
+    x = torch.full((2, 40, 8), 3.25)
+    x[1] = 0.0
+    b = _randn(8, seed=1)
+    dy = _randn(2, 40, 8, seed=2)
+    ref = R.group_norm(x, 2, None, b, 1e-5, 'silu', 0.2, dy)
+    leaf = x.to(device).requires_grad_(True)
+    y = ops.group_norm_act(leaf, 2, None, b.to(device))
+    R.check('y', y, *ref['y'])
+    R.check('dx', torch.autograd.grad(y, leaf, dy.to(device))[0], *ref['dx'])
+
+
+def test_empty(device):
+    from ag2video_amd import ops
+    w = torch.ones(8, device=device, requires_grad=True)
+    for shape in ((0, 5, 8), (3, 0, 8), (2, 0, 4, 8)):
+        x = torch.zeros(shape, device=device, requires_grad=True)
+        y = ops.group_norm_act(x, 2, w)
+        assert y.shape == x.shape
+        dx, dw = torch.autograd.grad(y.sum(), (x, w))
+        assert dx.shape == x.shape and not dw.any()
+    table = torch.ones(4, 0, device=device, requires_grad=True)
+    out = ops.embedding_scaled(torch.zeros(3, dtype=torch.long, device=device), table)
+    assert out.shape == (3, 0) and torch.autograd.grad(out.sum(), table)[0].shape == (4, 0)
+
+
+def test_group_norm_act_long_offsets(device):
+    """A map of more than 2^31 elements."""
+    from ag2video_amd import ops
+    N, S, C = 3, 1 << 20, 720
+    x = torch.empty(N, S, C, device=device, dtype=torch.bfloat16)
+    for n in range(N):
+        x[n].normal_(generator=torch.Generator(device=device).manual_seed(n))
+    y = ops.group_norm_act(x, 8, act='none')
+    for n in range(N):
+        ref = ops.group_norm_act(x[n:n + 1].clone(), 8, act='none')
+        assert torch.equal(ref[0, :1000], y[n, :1000]) and torch.equal(ref[0, -1000:], y[n, -1000:])
+    m = y[2].float().view(S, 8, 90).mean((0, 2))
+    assert m.abs().max() < 1e-3
+    del y, ref
+    leaf = x.requires_grad_(True)
+    y = ops.group_norm_act(leaf, 8, act='none')
+    (dx,) = torch.autograd.grad(y, leaf, x.detach())        # dy = x: what is left of it is rounding
+    assert dx[2, -1000:].float().abs().max() < 0.05 and dx[0, :1000].float().abs().max() < 0.05
+
+
+@pytest.mark.parametrize("S", [12, 6000])
+def test_group_norm_act_against_differences(S, device):
+    """The directional derivative by central differences of the operator itself: within the rounding of the two forward passes and the
+    difference quotient's own error, which the 64-bit reference gives."""
+    from ag2video_amd import ops
+    N, C, G, e = 2, 12, 3, 2.0 ** -6
+    x, w, b = _randn(N, S, C, seed=1), 1 + 0.2 * _randn(C, seed=2), _randn(C, seed=3)
+    dy = _randn(N, S, C, seed=4)
+    dirs = [_randn(*t.shape, seed=5 + i) for i, t in enumerate((x, w, b))]
+
+    def at(k):
+        return [t + k * e * d for t, d in zip((x, w, b), dirs)]
+
+    vals, refs, slack = [], [], 0.0
+    for k in (1, -1):
+        px, pw, pb = at(k)
+        y, bound = R.group_norm(px, G, pw, pb, 1e-5, 'silu', 0.2)['y']
+        refs.append(float((y * dy.double()).sum()))
+        slack += float((bound * dy.double().abs()).sum())
+        got = ops.group_norm_act(px.to(device), G, pw.to(device), pb.to(device))
+        vals.append(float((got.cpu().double() * dy.double()).sum()))
+    by_op, by_ref = (vals[0] - vals[1]) / (2 * e), (refs[0] - refs[1]) / (2 * e)
+    assert abs(by_op - by_ref) <= slack / (2 * e)
+    leaves = [t.to(device).requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(ops.group_norm_act(leaves[0], G, *leaves[1:]), leaves, dy.to(device))
+    ref = R.group_norm(x, G, w, b, 1e-5, 'silu', 0.2, dy)
+    along = sum(float((g.cpu().double() * d.double()).sum()) for g, d in zip(grads, dirs))
+    true = sum(float((ref[k][0] * d.double()).sum()) for k, d in zip(('dx', 'dweight', 'dbias'), dirs))
+    rounding = sum(float((ref[k][1] * d.double().abs()).sum()) for k, d in zip(('dx', 'dweight', 'dbias'), dirs))
+    assert abs(along - true) <= rounding
+    assert abs(along - by_op) <= rounding + slack / (2 * e) + abs(true - by_ref)
+
+
+def _chain(idx, table, w, b, groups=4):
+    from ag2video_amd import ops
+    rows = ops.embedding_scaled(idx, table, 3.0, 0)
+    return ops.group_norm_act(rows, groups, w, b)
+
+
+@pytest.mark.parametrize("shape", [(2, 6), (2, 9, 11), (3, 70, 64)], ids=str)
+def test_run_together(shape, device):
+    """A map of labels: its rows looked up, normalised over the map and activated, gradients back into the table."""
+    n = 1
+    for s in shape:
+        n *= s
+    V, D = 19, 32
+    idx = _tokens(n, V, 1).view(shape)
+    table, w, b = _randn(V, D, seed=2), 1 + 0.2 * _randn(D, seed=3), _randn(D, seed=4)
+    dy = _randn(*shape, D, seed=5)
+    leaves = [t.to(device).requires_grad_(True) for t in (table, w, b)]
+    y = _chain(idx.to(device), *leaves)
+    # the intermediate rows, as the operator rounds them, are the reference's input; the table's gradient takes the reference's dx with
+    # its bound through the sum
+    rows = (table.double()[idx] * 3.0).float()
+    ref = R.group_norm(rows, 4, w, b, 1e-5, 'silu', 0.2, dy)
+    R.check('y', y, *ref['y'])
+    dt, dw, db = torch.autograd.grad(y, leaves, dy.to(device))
+    R.check('dweight', dw, *ref['dweight'])
+    R.check('dbias', db, *ref['dbias'])
+    dx, e_dx = ref['dx']
+    at = idx.reshape(-1)
+    total = torch.zeros(V, D, dtype=torch.float64).index_add_(0, at, dx.reshape(-1, D)) * 3.0
+    off = torch.zeros(V, D, dtype=torch.float64).index_add_(0, at, (e_dx + R.DEPTH * R.U * dx.abs()).reshape(-1, D)) * 3.0
+    total[0], off[0] = 0.0, 0.0
+    R.check('dtable', dt, total, off * (1 + R.U) + 4 * R.U * total.abs())
+
+
+def test_other_stream_and_replay(device):
+    """Forward and backward on a side stream, then captured into a graph and replayed on new values between eager calls: the same bits."""
+    V, D, shape = 300, 48, (4, 900)
+    torch.manual_seed(0)
+    idx = torch.randint(V, shape, device=device)
+    fresh = [torch.randn(V, D, device=device), torch.randn(D, device=device), torch.randn(D, device=device)]
+    dys = [torch.randn(*shape, D, device=device) for _ in range(4)]
+
+    def step(idx, table, w, b, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (table, w, b)]
+        y = _chain(idx, *leaves)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    eager = step(idx, *fresh, dys[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = step(idx, *fresh, dys[0])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(eager, there))
+
+    s_idx, s_in, s_dy = idx.clone(), [t.clone() for t in fresh], dys[0].clone()
+    with torch.cuda.stream(side):
+        step(s_idx, *s_in, s_dy)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):                                     # two graphs, one memory pool
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            out = step(s_idx, *s_in, s_dy)
+        graphs.append(graph)
+        outs.append(out)
+    for k in range(4):
+        s_idx.copy_(torch.randint(V, shape, device=device, generator=torch.Generator(device=device).manual_seed(k)))
+        for t in s_in:
+            t.add_(0.25)
+        s_dy.copy_(dys[k])
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            got = [t.clone() for t in out]
+            torch.cuda.synchronize()
+            want = step(s_idx, *s_in, s_dy)
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_calls_on_two_streams_at_once(device):
+    torch.manual_seed(1)
+    idx = torch.randint(5000, (30000,), device=device)
+    table, x = torch.randn(5000, 40, device=device), torch.randn(4, 5000, 64, device=device)
+    dout, dy = torch.randn(30000, 40, device=device), torch.randn(4, 5000, 64, device=device)
+    from ag2video_amd import ops
+
+    def embed():
+        t = table.detach().requires_grad_(True)
+        return torch.autograd.grad(ops.embedding_scaled(idx, t, 1.5), t, dout)[0]
+
+    def norm():
+        t = x.detach().requires_grad_(True)
+        return torch.autograd.grad(ops.group_norm_act(t, 8), t, dy)[0]
+
+    want = embed(), norm()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for _ in range(3):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((k % 2, (embed, norm)[k % 2]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want[k]) for k, t in got)
+
+
+def test_modules(device):
+    """layers.Embedding with a scale and layers.GroupNormAct: the operators with nn.Embedding's and nn.GroupNorm's parameters."""
+    from ag2video_amd import ops
+    from ag2video_amd.models.layers import Embedding, GroupNormAct
+    emb = Embedding(11, 24, padding_idx=3, scale=2.0).to(device)
+    norm = GroupNormAct(4, 24, act='lrelu', slope=0.1).to(device)
+    assert set(norm.state_dict()) == {'weight', 'bias'} and set(emb.state_dict()) == {'weight'}
+    idx = _tokens(40, 11, 1).view(2, 20).to(device)
+    y = norm(emb(idx))
+    want = ops.group_norm_act(ops.embedding_scaled(idx, emb.weight, 2.0, 3), 4, norm.weight, norm.bias, act='lrelu', slope=0.1)
+    assert torch.equal(y, want)
+    y.square().sum().backward()
+    assert not emb.weight.grad[3].any() and emb.weight.grad[4].any() and norm.weight.grad.any()
+    plain = Embedding(11, 24).to(device)
+    assert torch.equal(plain(idx), ops.embedding(idx, plain.weight))
+    half = Embedding(11, 24).to(device).to(torch.bfloat16)
+    assert half(idx).dtype == torch.bfloat16
+
+
+def test_no_second_derivative(device):
+    from ag2video_amd import ops
+    x = torch.randn(2, 5, 8, device=device, requires_grad=True)
+    (g,) = torch.autograd.grad(ops.group_norm_act(x, 2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
