@@ -66,7 +66,8 @@ struct ElemF16 {
     static __device__ __forceinline__ void unpack(u32x4 r, float (&v)[8]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f16x2 h = __builtin_bit_cast(f16x2, r[i]);
+            const unsigned u = r[i];      // (a bit cast of the vector's element itself takes element 0)
+            const f16x2 h = __builtin_bit_cast(f16x2, u);
             v[2 * i] = (float)h[0];
             v[2 * i + 1] = (float)h[1];
         }

@@ -2,82 +2,597 @@
 //   out[i, :] = scale * table[idx_i, :]          dtable[v, :] = scale * sum over {i : idx_i = v} of dout[i, :]
 // A token outside [0, V) reads nothing: its row of the output is NaN, and it takes part in no sum; neither does padding_idx.  Products
 // and sums are in fp32 and rounded once.
+//
+// Both directions move memory and compute nothing to speak of: the lookup reads n rows (from the caches, where tokens repeat) and writes
+// n rows; the gradient reads n rows and writes V.
+//
+// The gradient, by sizes:
+//   few rows, few tokens    one launch: a workgroup per row of the table picks its tokens out of all n (embed_pick_kernel);
+//   up to RANK_MAX tokens   a token's place in the sorted order is the number of tokens before it: n^2 / 64 compares on the ballot path,
+//                           spread over the whole chip in ONE launch that also clears the table's gradient (embed_rank_kernel);
+//   more                    a stable radix sort, 9 bits a pass, two launches a pass (embed_hist_kernel, embed_scatter_kernel).
+// After a sort, embed_sum_kernel walks equal shares of the sorted order -- a long run of one token costs no more than many short ones --
+// and writes every row whose tokens lie inside one workgroup's share; embed_join_kernel adds the rest up, in order.  No atomics on
+// floating-point values: equal calls give equal bits.
 #include "elem.h"
 
 __device__ __forceinline__ long long token_at(const void* idx, int wide, long long stride, long long i) {
     return wide ? ((const long long*)idx)[i * stride] : (long long)((const int*)idx)[i * stride];
 }
-
-template <class E>
-__global__ __launch_bounds__(256) void embed_fwd_kernel(const void* idx, int wide, long long istride, const typename E::T* table,
-                                                        long long tstride, typename E::T* out, long long n, long long V, int D, float scale) {
-    for (long long i = blockIdx.x; i < n; i += gridDim.x) {
-        const long long v = token_at(idx, wide, istride, i);
-        const bool in = v >= 0 && v < V;
-        for (int d = threadIdx.x; d < D; d += 256)
-            out[i * D + d] = E::narrow(in ? scale * E::widen(table[v * tstride + d]) : __builtin_nanf(""));
-    }
+// sort key of a token: V for the ones that take part in no sum
+__device__ __forceinline__ int key_at(const void* idx, int wide, long long stride, long long i, int V, int pad) {
+    const long long v = token_at(idx, wide, stride, i);
+    return v >= 0 && v < V && v != pad ? (int)v : V;
 }
 
-// one workgroup per row of the table
+// ---------------------------------------------------------------- lookup
+// 2^lsh lanes a row, 16 bytes a lane, four rows in flight a thread.  The last vector of a row whose width is no multiple of the vector
+// moves back to end with the row (its first elements are then written twice, with the same values), so every access is 16 bytes wide.
 template <class E>
-__global__ __launch_bounds__(256) void embed_bwd_kernel(const void* idx, int wide, long long istride, const typename E::T* dout, long long dstride,
-                                                        typename E::T* dtable, long long n, long long V, int D, float scale, long long pad) {
-    const long long v = blockIdx.x;
-    for (int d0 = 0; d0 < D; d0 += 256) {
-        const int d = d0 + threadIdx.x;
-        float acc = 0.f;
-        if (d < D) {
-            if (v != pad)
-                for (long long i = 0; i < n; ++i)
-                    if (token_at(idx, wide, istride, i) == v) acc += E::widen(dout[i * dstride + d]);
-            dtable[v * D + d] = E::narrow(scale * acc);
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__ idx, int wide, long long istride,
+                                                        const typename E::T* __restrict__ table, long long tstride,
+                                                        typename E::T* __restrict__ out, long long n, int V, int D, float scale, int lsh) {
+    constexpr int U = 4;
+    const int lane = threadIdx.x & ((1 << lsh) - 1), grp = threadIdx.x >> lsh, ng = 256 >> lsh;
+    for (long long i0 = (long long)blockIdx.x * ng * U + grp; i0 < n; i0 += (long long)gridDim.x * ng * U) {
+        long long row[U];
+        bool in[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long i = i0 + u * ng;
+            const long long v = i < n ? token_at(idx, wide, istride, i) : 0;
+            in[u] = v >= 0 && v < V;
+            row[u] = (in[u] ? v : 0) * tstride;
+        }
+        for (int c0 = lane * E::V; c0 < D; c0 += E::V << lsh) {
+            const int c = D < E::V ? 0 : min(c0, D - E::V);
+            u32x4 r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i0 + u * ng < n) r[u] = load_vec<E>(table + row[u] + c, D);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float v[E::V];
+                E::unpack(r[u], v);
+#pragma unroll
+                for (int k = 0; k < E::V; ++k) v[k] = in[u] ? v[k] * scale : __builtin_nanf("");
+                if (i0 + u * ng < n) store_vec<E>(out + (i0 + u * ng) * D + c, D, v);
+            }
         }
     }
 }
 
+// ---------------------------------------------------------------- gradient: one launch for few rows and few tokens
+#define PICK_MAX 4096
+template <class E>
+__global__ __launch_bounds__(256) void embed_pick_kernel(const void* __restrict__ idx, int wide, long long istride,
+                                                         const typename E::T* __restrict__ dout, long long dstride,
+                                                         typename E::T* __restrict__ dtable, int n, int V, int D, float scale, int pad, int lsh) {
+    __shared__ int list[PICK_MAX], cnt[4];
+    __shared__ float part[256 * E::V];
+    const int v = blockIdx.x % V, slice = blockIdx.x / V;
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
+    // each wave lists the tokens of its quarter, in order
+    const int quarter = (n + 3) / 4, lo = wave * quarter, hi = min(n, lo + quarter);
+    int* mine = list + wave * (PICK_MAX / 4);
+    int found = 0;
+    for (int b = lo; b < hi; b += 64) {
+        const int i = b + wl;
+        const bool hit = i < hi && key_at(idx, wide, istride, i, V, pad) == v;
+        const unsigned long long m = __ballot(hit);
+        if (hit) mine[found + __popcll(m & ((1ull << wl) - 1))] = i;
+        found += __popcll(m);
+    }
+    if (wl == 0) cnt[wave] = found;
+    __syncthreads();
+    const int c1 = cnt[0], c2 = c1 + cnt[1], c3 = c2 + cnt[2], total = c3 + cnt[3];
+    const int lane = threadIdx.x & ((1 << lsh) - 1), grp = threadIdx.x >> lsh, ng = 256 >> lsh;
+    const int c0 = (slice << lsh) * E::V + lane * E::V, c = D < E::V ? 0 : min(c0, D - E::V);
+    const int share = (total + ng - 1) / ng, e1 = min(total, (grp + 1) * share);
+    float acc[E::V] = {};
+    if (c0 < D)
+        for (int e = grp * share; e < e1; e += 4) {
+            u32x4 r[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int q = e + u;
+                if (q < e1) {
+                    const int i = q < c1 ? list[q] : q < c2 ? list[PICK_MAX / 4 + q - c1] : q < c3 ? list[PICK_MAX / 2 + q - c2] : list[3 * (PICK_MAX / 4) + q - c3];
+                    r[u] = load_vec<E>(dout + (long long)i * dstride + c, D);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (e + u < e1) {
+                    float x[E::V];
+                    E::unpack(r[u], x);
+#pragma unroll
+                    for (int k = 0; k < E::V; ++k) acc[k] += x[k];
+                }
+        }
+#pragma unroll
+    for (int k = 0; k < E::V; ++k) part[k * 256 + threadIdx.x] = acc[k];
+    __syncthreads();
+    if (grp == 0 && c0 < D) {
+        for (int g = 1; g < ng; ++g)
+#pragma unroll
+            for (int k = 0; k < E::V; ++k) acc[k] += part[k * 256 + (g << lsh) + lane];
+#pragma unroll
+        for (int k = 0; k < E::V; ++k) acc[k] *= scale;
+        store_vec<E>(dtable + (long long)v * D + c, D, acc);
+    }
+}
+
+// ---------------------------------------------------------------- gradient: clearing the table (rows that no token names)
+__device__ __forceinline__ void clear_share(char* p, long long bytes, int blk, int nblk) {
+    const long long vecs = bytes >> 4;
+    const u32x4 z = {0, 0, 0, 0};
+    for (long long i = (long long)blk * blockDim.x + threadIdx.x; i < vecs; i += (long long)nblk * blockDim.x)
+        reinterpret_cast<u32x4_a2*>(p)[i] = z;
+    if (blk == 0)
+        for (long long i = (vecs << 4) + threadIdx.x * 2; i < bytes; i += blockDim.x * 2) *reinterpret_cast<unsigned short*>(p + i) = 0;
+}
+
+// ---------------------------------------------------------------- gradient: the order by counting
+// Workgroup b ranks tokens [b * RANK_T, ...): rank_i = #{j : k_j < k_i} + #{j < i : k_j = k_i}.  A lane holds k_j, k_i is uniform: a
+// compare and a scalar bit count per 64 pairs.  Tiles of j wholly before i count k_j <= k_i, tiles wholly behind k_j < k_i.
+// Workgroups beyond the ranking ones clear the table's gradient.
+#define RANK_MAX 8192
+#define RANK_T 32
+__global__ __launch_bounds__(256) void embed_rank_kernel(const void* __restrict__ idx, int wide, long long istride, int* __restrict__ skey,
+                                                         int* __restrict__ order, int n, int V, int pad, int rank_blocks, char* clear,
+                                                         long long clear_bytes) {
+    if ((int)blockIdx.x >= rank_blocks) {
+        clear_share(clear, clear_bytes, blockIdx.x - rank_blocks, gridDim.x - rank_blocks);
+        return;
+    }
+    __shared__ int sh[4][RANK_T];
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, i0 = blockIdx.x * RANK_T;
+    int ki[RANK_T], cnt[RANK_T];
+#pragma unroll
+    for (int t = 0; t < RANK_T; ++t) {
+        ki[t] = __builtin_amdgcn_readfirstlane(i0 + t < n ? key_at(idx, wide, istride, i0 + t, V, pad) : 0);
+        cnt[t] = 0;
+    }
+    for (int j0 = wave * 64; j0 < n; j0 += 256) {
+        const int j = j0 + wl;
+        const int kj = j < n ? key_at(idx, wide, istride, j, V, pad) : 0x7fffffff;
+        if (j0 + 64 <= i0) {                   // wholly before: equal ones count
+#pragma unroll
+            for (int t = 0; t < RANK_T; ++t) cnt[t] += __popcll(__ballot(kj <= ki[t]));
+        } else if (j0 >= i0 + RANK_T) {        // wholly behind
+#pragma unroll
+            for (int t = 0; t < RANK_T; ++t) cnt[t] += __popcll(__ballot(kj < ki[t]));
+        } else {
+#pragma unroll
+            for (int t = 0; t < RANK_T; ++t) cnt[t] += __popcll(__ballot(kj < ki[t] || (kj == ki[t] && j < i0 + t)));
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RANK_T; ++t)
+        if (wl == t) sh[wave][t] = cnt[t];
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (t < RANK_T && i0 + t < n) {
+        const int r = sh[0][t] + sh[1][t] + sh[2][t] + sh[3][t];
+        skey[r] = key_at(idx, wide, istride, i0 + t, V, pad);
+        order[r] = i0 + t;
+    }
+}
+
+// ---------------------------------------------------------------- gradient: the order by radix passes
+// A pass sorts by `bits` <= 9 bits of the key, stably.  Each workgroup owns `rounds` * 2048 consecutive entries.  hist: how often each digit
+// occurs in each workgroup's share, counts[digit][workgroup].  scatter: a workgroup reads all counts, which gives where its entries of
+// each digit begin, ranks its entries (within a wave by matching digits over ballots, then over waves, then over rounds) and writes them.
+#define RADIX_BITS 9
+#define RADIX_N (1 << RADIX_BITS)
+#define RADIX_THREADS 512
+#define RADIX_TILE 2048
+#define RADIX_BLOCKS 128
+struct RadixSrc {
+    const void* idx;          // first pass: the tokens
+    int wide, V, pad;
+    long long istride;
+    const int *key, *pos;     // later passes
+};
+__device__ __forceinline__ int radix_key(const RadixSrc& s, int e) { return s.key ? s.key[e] : key_at(s.idx, s.wide, s.istride, e, s.V, s.pad); }
+
+__global__ __launch_bounds__(RADIX_THREADS) void embed_hist_kernel(RadixSrc s, int n, int shift, int bits, int rounds, int nb, int* __restrict__ counts,
+                                                                   char* clear, long long clear_bytes) {
+    if ((int)blockIdx.x >= nb) {
+        clear_share(clear, clear_bytes, blockIdx.x - nb, gridDim.x - nb);
+        return;
+    }
+    __shared__ int h[RADIX_N];
+    h[threadIdx.x] = 0;
+    __syncthreads();
+    const int mask = (1 << bits) - 1;
+    const long long lo = (long long)blockIdx.x * rounds * RADIX_TILE, hi = min((long long)n, lo + (long long)rounds * RADIX_TILE);
+    for (long long e = lo + threadIdx.x; e < hi; e += RADIX_THREADS) atomicAdd(&h[(radix_key(s, (int)e) >> shift) & mask], 1);   // whole numbers: any order, one result
+    __syncthreads();
+    if (threadIdx.x <= mask) counts[threadIdx.x * nb + blockIdx.x] = h[threadIdx.x];
+}
+
+__global__ __launch_bounds__(RADIX_THREADS) void embed_scatter_kernel(RadixSrc s, int n, int shift, int bits, int rounds, int nb,
+                                                                      const int* __restrict__ counts, int* __restrict__ okey, int* __restrict__ opos) {
+    constexpr int W = RADIX_THREADS / 64, PER = RADIX_TILE / RADIX_THREADS;
+    __shared__ int cnt[W][RADIX_N], base[RADIX_N], wsum[W];
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, mask = (1 << bits) - 1, d = threadIdx.x;
+    // where this workgroup's entries of digit d begin: all entries of smaller digits, then those of d in earlier workgroups
+    int before = 0, total = 0;
+    if (d <= mask)
+        for (int b = 0; b < nb; ++b) {
+            const int c = counts[d * nb + b];
+            total += c;
+            before += b < (int)blockIdx.x ? c : 0;
+        }
+    int scan = total;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(scan, o, 64);
+        if (wl >= o) scan += up;
+    }
+    if (wl == 63) wsum[wave] = scan;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) scan += wsum[w];
+    base[d] = scan - total + before;
+    for (int r = 0; r < rounds; ++r) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) cnt[w][d] = 0;
+        __syncthreads();
+        const long long e0 = ((long long)blockIdx.x * rounds + r) * RADIX_TILE + wave * (64 * PER);
+        int key[PER], pos[PER], rank[PER];
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const long long e = e0 + q * 64 + wl;
+            const bool in = e < n;
+            key[q] = in ? radix_key(s, (int)e) : 0;
+            pos[q] = in ? (s.pos ? s.pos[e] : (int)e) : 0;
+        }
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const bool in = e0 + q * 64 + wl < n;
+            const int dig = (key[q] >> shift) & mask;
+            unsigned long long m = __ballot(in);
+            for (int b = 0; b < bits; ++b) {
+                const bool bit = (dig >> b) & 1;
+                const unsigned long long same = __ballot(bit);
+                m &= bit ? same : ~same;
+            }
+            const int lower = __popcll(m & ((1ull << wl) - 1));
+            int seen = 0;
+            if (in) seen = cnt[wave][dig];
+            __builtin_amdgcn_wave_barrier();
+            if (in && lower == 0) cnt[wave][dig] = seen + __popcll(m);
+            __builtin_amdgcn_wave_barrier();
+            rank[q] = seen + lower;
+        }
+        __syncthreads();
+        int run = base[d];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const int c = cnt[w][d];
+            cnt[w][d] = run;
+            run += c;
+        }
+        base[d] = run;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < PER; ++q)
+            if (e0 + q * 64 + wl < n) {
+                const int at = cnt[wave][(key[q] >> shift) & mask] + rank[q];
+                okey[at] = key[q];
+                opos[at] = pos[q];
+            }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- gradient: sums over the sorted order
+// A group of 2^lsh lanes walks L sorted entries, eight rows in flight.  A segment (the entries of one token) that begins and ends in its
+// share goes to the table at once; the part of one that began earlier (head) or goes on (tail) goes to LDS, where one group joins them in
+// order; what began before the workgroup or goes on behind it goes to part[0 / 1][workgroup][:] for embed_join_kernel.
+struct SumArgs {
+    const int *skey, *order;
+    const void* dout;
+    void* dtable;
+    float* part;
+    long long dstride;
+    int n, V, D, lsh, L, nblk;
+    float scale;
+};
+template <class E>
+__global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
+    constexpr int U = 8;
+    __shared__ float head[256 * E::V], tail[256 * E::V];
+    __shared__ int flags[32], fkey[32], lkey[32];
+    const int lane = threadIdx.x & ((1 << a.lsh) - 1), grp = threadIdx.x >> a.lsh, ng = 256 >> a.lsh;
+    const int blk = blockIdx.x % a.nblk, slice = blockIdx.x / a.nblk;
+    const int c0 = ((slice << a.lsh) + lane) * E::V, c = a.D < E::V ? 0 : min(c0, a.D - E::V);
+    const bool mine = c0 < a.D;
+    const typename E::T* dout = (const typename E::T*)a.dout + c;
+    typename E::T* dtable = (typename E::T*)a.dtable + c;
+    const long long e0 = ((long long)blk * ng + grp) * a.L, e1 = min((long long)a.n, e0 + a.L);
+    if (e0 < e1) {
+        int cur = a.skey[e0];
+        const int first = cur;
+        bool began_before = e0 > 0 && a.skey[e0 - 1] == cur;
+        const int next = e1 < a.n ? a.skey[e1] : -1;
+        int f = began_before ? 1 : 0;
+        float acc[E::V] = {};
+        auto finish = [&]() {          // the segment `cur` ends here
+            if (began_before) {
+#pragma unroll
+                for (int k = 0; k < E::V; ++k) head[k * 256 + threadIdx.x] = acc[k];
+            } else if (cur != a.V && mine) {
+                float v[E::V];
+#pragma unroll
+                for (int k = 0; k < E::V; ++k) v[k] = acc[k] * a.scale;
+                store_vec<E>(dtable + (long long)cur * a.D, a.D, v);
+            }
+        };
+        for (long long e = e0; e < e1; e += U) {
+            int key[U], pos[U];
+#pragma unroll
+            for (int q = 0; q < U / 4; ++q) {
+                const int4 k4 = *reinterpret_cast<const int4*>(a.skey + e + 4 * q), p4 = *reinterpret_cast<const int4*>(a.order + e + 4 * q);
+                key[4 * q] = k4.x; key[4 * q + 1] = k4.y; key[4 * q + 2] = k4.z; key[4 * q + 3] = k4.w;
+                pos[4 * q] = p4.x; pos[4 * q + 1] = p4.y; pos[4 * q + 2] = p4.z; pos[4 * q + 3] = p4.w;
+            }
+            u32x4 r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (e + u < e1 && key[u] != a.V && mine) r[u] = load_vec<E>(dout + pos[u] * a.dstride, a.D);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (e + u < e1) {
+                    if (key[u] != cur) {
+                        finish();
+                        cur = key[u];
+                        began_before = false;
+#pragma unroll
+                        for (int k = 0; k < E::V; ++k) acc[k] = 0.f;
+                    }
+                    if (key[u] != a.V && mine) {
+                        float x[E::V];
+                        E::unpack(r[u], x);
+#pragma unroll
+                        for (int k = 0; k < E::V; ++k) acc[k] += x[k];
+                    }
+                }
+        }
+        if (next != cur) {
+            finish();
+        } else if (began_before) {     // one segment fills the share and goes on
+            f |= 2;
+#pragma unroll
+            for (int k = 0; k < E::V; ++k) head[k * 256 + threadIdx.x] = acc[k];
+        } else {
+            f |= 4;
+#pragma unroll
+            for (int k = 0; k < E::V; ++k) tail[k * 256 + threadIdx.x] = acc[k];
+        }
+        if (lane == 0) { flags[grp] = f; fkey[grp] = first; lkey[grp] = cur; }
+    } else if (lane == 0) {
+        flags[grp] = 0;
+    }
+    __syncthreads();
+    if (grp != 0 || !mine) return;
+    float acc[E::V] = {};
+    bool open = false, outside = false;
+    float* part = a.part + (long long)blk * a.D + c;
+    const long long half = (long long)a.nblk * a.D;
+    auto spill = [&](float* to) {
+#pragma unroll
+        for (int k = 0; k < E::V; ++k)
+            if (k < a.D) to[k] = acc[k];
+    };
+    for (int g = 0; g < ng; ++g) {
+        const int f = flags[g], at = (g << a.lsh) + lane;
+        if (f & 1) {
+            if (!open) { open = outside = true; }
+#pragma unroll
+            for (int k = 0; k < E::V; ++k) acc[k] += head[k * 256 + at];
+            if (!(f & 2)) {
+                if (outside) {
+                    spill(part);
+                } else if (fkey[g] != a.V) {
+                    float v[E::V];
+#pragma unroll
+                    for (int k = 0; k < E::V; ++k) v[k] = acc[k] * a.scale;
+                    store_vec<E>(dtable + (long long)fkey[g] * a.D, a.D, v);
+                }
+                open = false;
+            }
+        }
+        if (f & 4) {
+            open = true;
+            outside = false;
+#pragma unroll
+            for (int k = 0; k < E::V; ++k) acc[k] = tail[k * 256 + at];
+        }
+    }
+    if (open) spill(outside ? part : part + half);
+}
+
+// The segments that cross workgroups of embed_sum_kernel: the workgroup where one begins adds its tail and the heads behind it.
+template <class E>
+__global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
+    __shared__ float sh[256 * E::V];
+    const int blk = blockIdx.x % a.nblk, slice = blockIdx.x / a.nblk, ng = 256 >> a.lsh;
+    const long long B = (long long)ng * a.L, s = blk * B, t = min((long long)a.n, s + B) - 1;
+    if (t + 1 >= a.n) return;
+    const int key = a.skey[t];
+    if (key == a.V || a.skey[t + 1] != key) return;
+    if (a.skey[s] == key && s > 0 && a.skey[s - 1] == key) return;       // began earlier
+    int m = 0;                                                           // workgroups behind this one that the segment reaches
+    for (int q = blk + 1;; q += 256) {
+        const int k = __syncthreads_count(q + (int)threadIdx.x < a.nblk && a.skey[(q + (int)threadIdx.x) * B] == key);
+        m += k;
+        if (k < 256) break;
+    }
+    const int lane = threadIdx.x & ((1 << a.lsh) - 1), grp = threadIdx.x >> a.lsh;
+    const int c0 = ((slice << a.lsh) + lane) * E::V, c = a.D < E::V ? 0 : min(c0, a.D - E::V);
+    const int share = (m + ng - 1) / ng, q0 = min(m, grp * share), q1 = min(m, q0 + share);
+    const float* heads = a.part + (long long)(blk + 1) * a.D + c;
+    float acc[E::V] = {};
+    if (c0 < a.D) {
+        for (int q = q0; q < q1; q += 4) {
+            float x[4][E::V];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int k = 0; k < E::V; ++k) x[u][k] = q + u < q1 && k < a.D ? heads[(long long)(q + u) * a.D + k] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int k = 0; k < E::V; ++k) acc[k] += x[u][k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < E::V; ++k) sh[k * 256 + threadIdx.x] = acc[k];
+    __syncthreads();
+    if (grp == 0 && c0 < a.D) {
+        const float* tail = a.part + (long long)a.nblk * a.D + (long long)blk * a.D + c;
+        float v[E::V];
+#pragma unroll
+        for (int k = 0; k < E::V; ++k) v[k] = (k < a.D ? tail[k] : 0.f) + acc[k];
+        for (int g = 1; g < ng; ++g)
+#pragma unroll
+            for (int k = 0; k < E::V; ++k) v[k] += sh[k * 256 + (g << a.lsh) + lane];
+#pragma unroll
+        for (int k = 0; k < E::V; ++k) v[k] *= a.scale;
+        store_vec<E>((typename E::T*)a.dtable + (long long)key * a.D + c, a.D, v);
+    }
+}
+
+// ---------------------------------------------------------------- host
 static bool embed_ok(int dtype, int idx_bytes, long long n, long long V, int D) {
-    return dtype >= AG2V_F32 && dtype <= AG2V_F16 && (idx_bytes == 4 || idx_bytes == 8) && n > 0 && n < (1LL << 31) && V > 0 && V < (1LL << 31) && D > 0;
+    return dtype >= AG2V_F32 && dtype <= AG2V_F16 && (idx_bytes == 4 || idx_bytes == 8) && n > 0 && n < (1LL << 31) && V > 0 && V < (1LL << 31) - 1 && D > 0;
+}
+static int log2_up(long long v) {
+    int l = 0;
+    while ((1LL << l) < v) ++l;
+    return l;
+}
+static int vec_of(int dtype) { return dtype == AG2V_F32 ? ElemF32::V : ElemBF16::V; }
+
+// How the gradient of (n, V, D) runs.
+struct EmbedPlan {
+    bool pick, rank;
+    int lsh, slices, L, nblk;       // sums
+    int passes, bits, rounds, nb;   // radix
+    long long npad, words;          // workspace: sorted keys and positions, their ping-pong, counts, parts
+};
+static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
+    EmbedPlan p = {};
+    const long long cv = ((long long)D + vec_of(dtype) - 1) / vec_of(dtype);
+    p.lsh = log2_up(cv < 64 ? cv : 64);
+    if (p.lsh < 3) p.lsh = 3;       // at most 32 groups a workgroup
+    p.slices = (int)((cv + (1 << p.lsh) - 1) >> p.lsh);
+    p.pick = n <= PICK_MAX && V * p.slices <= 2048 && n * V <= (1LL << 20);
+    if (p.pick) return p;
+    p.rank = n <= RANK_MAX;
+    // entries a group walks: enough groups for 4096 waves, 8 .. 64; more only where the workgroups' parts would pass 16384
+    const int ng = 256 >> p.lsh;
+    long long L = (n * p.slices << p.lsh) / 64 / 4096;
+    L = L < 8 ? 8 : L > 64 ? 64 : 1LL << (log2_up(L + 1) - 1);
+    while ((n + ng * L - 1) / (ng * L) > 16384) L *= 2;
+    p.L = (int)L;
+    p.nblk = (int)((n + ng * L - 1) / (ng * L));
+    p.npad = (n + 63) / 64 * 64;
+    p.words = 2 * p.npad + 2LL * p.nblk * D;
+    if (!p.rank) {
+        const int all = log2_up(V + 1);      // keys 0 .. V
+        p.passes = (all + RADIX_BITS - 1) / RADIX_BITS;
+        p.bits = (all + p.passes - 1) / p.passes;
+        const long long tiles = (n + RADIX_TILE - 1) / RADIX_TILE;
+        p.rounds = (int)((tiles + RADIX_BLOCKS - 1) / RADIX_BLOCKS);
+        p.nb = (int)((tiles + p.rounds - 1) / p.rounds);
+        p.words += (p.passes > 1 ? 2 * p.npad : 0) + (long long)RADIX_N * p.nb;
+    }
+    return p;
 }
 
 template <class E>
-static int run_fwd(const void* idx, int idx_bytes, long long istride, const void* table, long long tstride, void* out, long long n, long long V,
-                   int D, float scale, hipStream_t st) {
-    const int grid = (int)(n < (1 << 20) ? n : (1 << 20));
-    hipLaunchKernelGGL(embed_fwd_kernel<E>, dim3(grid), dim3(256), 0, st, idx, idx_bytes == 8, istride, (const typename E::T*)table, tstride,
-                       (typename E::T*)out, n, V, D, scale);
+static int run_fwd(const void* idx, int idx_bytes, long long istride, const void* table, long long tstride, void* out, long long n, int V, int D,
+                   float scale, hipStream_t st) {
+    const long long cv = ((long long)D + E::V - 1) / E::V;
+    const int lsh = log2_up(cv < 64 ? cv : 64), rows = (256 >> lsh) * 4;
+    const long long blocks = (n + rows - 1) / rows;
+    hipLaunchKernelGGL(embed_fwd_kernel<E>, dim3((int)(blocks < (1 << 20) ? blocks : (1 << 20))), dim3(256), 0, st, idx, idx_bytes == 8, istride,
+                       (const typename E::T*)table, tstride, (typename E::T*)out, n, V, D, scale, lsh);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
+
 template <class E>
-static int run_bwd(const void* idx, int idx_bytes, long long istride, const void* dout, long long dstride, void* dtable, long long n, long long V,
-                   int D, float scale, long long pad, hipStream_t st) {
-    if (V >= (1LL << 24)) return AG2V_EINVAL;
-    hipLaunchKernelGGL(embed_bwd_kernel<E>, dim3((int)V), dim3(256), 0, st, idx, idx_bytes == 8, istride, (const typename E::T*)dout, dstride,
-                       (typename E::T*)dtable, n, V, D, scale, pad);
+static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istride, const void* dout, long long dstride, void* dtable, int n, int V,
+                   int D, float scale, int pad, float* workspace, hipStream_t st) {
+    if (p.pick) {
+        hipLaunchKernelGGL(embed_pick_kernel<E>, dim3(V * p.slices), dim3(256), 0, st, idx, wide, istride, (const typename E::T*)dout, dstride,
+                           (typename E::T*)dtable, n, V, D, scale, pad, p.lsh);
+        AG2V_CHECK_LAUNCH();
+        return AG2V_OK;
+    }
+    int *skey = (int*)workspace, *order = skey + p.npad;
+    const long long bytes = (long long)V * D * (long long)sizeof(typename E::T);
+    const long long cb = (bytes / 16 + 255) / 256;
+    const int clearers = cb < 1 ? 1 : cb < 1024 ? (int)cb : 1024;
+    SumArgs a = {skey, order, dout, dtable, (float*)(order + p.npad), dstride, n, V, D, p.lsh, p.L, p.nblk, scale};
+    if (p.rank) {
+        const int rank_blocks = ceil_div(n, RANK_T);
+        hipLaunchKernelGGL(embed_rank_kernel, dim3(rank_blocks + clearers), dim3(256), 0, st, idx, wide, istride, skey, order, n, V, pad, rank_blocks,
+                           (char*)dtable, bytes);
+        AG2V_CHECK_LAUNCH();
+    } else {
+        int* counts = (int*)(a.part + 2LL * p.nblk * D);
+        int *key2 = counts + (long long)RADIX_N * p.nb, *pos2 = key2 + p.npad;
+        RadixSrc s = {idx, wide, V, pad, istride, nullptr, nullptr};
+        for (int q = 0; q < p.passes; ++q) {
+            const bool last = ((p.passes - 1 - q) & 1) == 0;         // the last pass writes skey / order, the passes before it in turn
+            int *ok = last ? skey : key2, *op = last ? order : pos2;
+            hipLaunchKernelGGL(embed_hist_kernel, dim3(p.nb + (q == 0 ? clearers : 0)), dim3(RADIX_THREADS), 0, st, s, n, q * p.bits, p.bits, p.rounds,
+                               p.nb, counts, (char*)dtable, bytes);
+            AG2V_CHECK_LAUNCH();
+            hipLaunchKernelGGL(embed_scatter_kernel, dim3(p.nb), dim3(RADIX_THREADS), 0, st, s, n, q * p.bits, p.bits, p.rounds, p.nb, counts, ok, op);
+            AG2V_CHECK_LAUNCH();
+            s.key = ok;
+            s.pos = op;
+        }
+    }
+    hipLaunchKernelGGL(embed_sum_kernel<E>, dim3(p.nblk * p.slices), dim3(256), 0, st, a);
     AG2V_CHECK_LAUNCH();
+    if (p.nblk > 1) {
+        hipLaunchKernelGGL(embed_join_kernel<E>, dim3(p.nblk * p.slices), dim3(256), 0, st, a);
+        AG2V_CHECK_LAUNCH();
+    }
     return AG2V_OK;
 }
 
 extern "C" size_t ag2v_embed_bwd_workspace_floats(int dtype, long long n, long long V, int D) {
-    if (!embed_ok(dtype, 8, n, V, D)) return 0;
-    return 0;
+    return embed_ok(dtype, 8, n, V, D) ? (size_t)plan_of(dtype, n, V, D).words : 0;
 }
 extern "C" int ag2v_embed_fwd(int dtype, const void* idx, int idx_bytes, long long idx_stride, const void* table, long long table_stride,
                               void* out, long long n, long long V, int D, float scale, void* stream) {
     if (!idx || !table || !out || !embed_ok(dtype, idx_bytes, n, V, D) || table_stride < D) return AG2V_EINVAL;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == AG2V_F32) return run_fwd<ElemF32>(idx, idx_bytes, idx_stride, table, table_stride, out, n, V, D, scale, st);
-    if (dtype == AG2V_BF16) return run_fwd<ElemBF16>(idx, idx_bytes, idx_stride, table, table_stride, out, n, V, D, scale, st);
-    return run_fwd<ElemF16>(idx, idx_bytes, idx_stride, table, table_stride, out, n, V, D, scale, st);
+    if (dtype == AG2V_F32) return run_fwd<ElemF32>(idx, idx_bytes, idx_stride, table, table_stride, out, n, (int)V, D, scale, st);
+    if (dtype == AG2V_BF16) return run_fwd<ElemBF16>(idx, idx_bytes, idx_stride, table, table_stride, out, n, (int)V, D, scale, st);
+    return run_fwd<ElemF16>(idx, idx_bytes, idx_stride, table, table_stride, out, n, (int)V, D, scale, st);
 }
 extern "C" int ag2v_embed_bwd(int dtype, const void* idx, int idx_bytes, long long idx_stride, const void* dout, long long dout_stride,
                               void* dtable, long long n, long long V, int D, float scale, long long padding_idx, float* workspace,
                               size_t workspace_floats, void* stream) {
     if (!idx || !dout || !dtable || !embed_ok(dtype, idx_bytes, n, V, D)) return AG2V_EINVAL;
-    if (workspace_floats < ag2v_embed_bwd_workspace_floats(dtype, n, V, D)) return AG2V_EINVAL;
+    const EmbedPlan p = plan_of(dtype, n, V, D);
+    if ((p.words && !workspace) || workspace_floats < (size_t)p.words || ((uintptr_t)workspace & 15)) return AG2V_EINVAL;
+    if ((long long)p.nblk * p.slices >= (1LL << 24)) return AG2V_EINVAL;
+    const int wide = idx_bytes == 8, pad = padding_idx >= 0 && padding_idx < V ? (int)padding_idx : -1;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == AG2V_F32) return run_bwd<ElemF32>(idx, idx_bytes, idx_stride, dout, dout_stride, dtable, n, V, D, scale, padding_idx, st);
-    if (dtype == AG2V_BF16) return run_bwd<ElemBF16>(idx, idx_bytes, idx_stride, dout, dout_stride, dtable, n, V, D, scale, padding_idx, st);
-    return run_bwd<ElemF16>(idx, idx_bytes, idx_stride, dout, dout_stride, dtable, n, V, D, scale, padding_idx, st);
+    if (dtype == AG2V_F32)
+        return run_bwd<ElemF32>(p, idx, wide, idx_stride, dout, dout_stride, dtable, (int)n, (int)V, D, scale, pad, workspace, st);
+    if (dtype == AG2V_BF16)
+        return run_bwd<ElemBF16>(p, idx, wide, idx_stride, dout, dout_stride, dtable, (int)n, (int)V, D, scale, pad, workspace, st);
+    return run_bwd<ElemF16>(p, idx, wide, idx_stride, dout, dout_stride, dtable, (int)n, (int)V, D, scale, pad, workspace, st);
 }
