@@ -2509,7 +2509,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act='silu', slop
     ``weight`` / ``bias``: [C] in x's type or fp32, each may be None.  ``act``: 'silu', 'lrelu' (``slope``; 0 = relu) or 'none'.  Views whose
     channels are adjacent are read in place (a channel slice; ``t.permute(0, 2, 3, 1)`` of a channels-last NCHW tensor).  Gradients for x,
     weight and bias; h and the activation's derivative are computed again from x, so the tape holds x and two numbers per group.  Sums in
-    fp32 in a fixed order (no atomics)."""
+    fp32 in a fixed order (no atomics); y and dx of a sample do not depend on the rest of the batch."""
     _elem_chk('group_norm_act', x)
     if x.dim() < 2 or x.shape[-1] == 0:
         raise RuntimeError("group_norm_act: expected x [N, ..., C > 0], got %s" % (tuple(x.shape),))
@@ -2521,8 +2521,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act='silu', slop
     eps, slope = float(eps), float(slope)
     if not 0.0 <= eps < float('inf') or slope != slope:
         raise RuntimeError("group_norm_act: eps %r, slope %r" % (eps, slope))
-    if max(x.shape[0] * groups, x.shape[0] and x[0].numel() // C, C) >= _INT_LIMIT:
-        raise RuntimeError("group_norm_act: %s in %d groups: at most 2^31 - 1 (sample, group) pairs, positions and channels" % (tuple(x.shape), groups))
+    if x.shape[0] * groups >= 1 << 24 or max(x.shape[0] and x[0].numel() // C, C) >= _INT_LIMIT:
+        raise RuntimeError("group_norm_act: %s in %d groups: fewer than 2^24 (sample, group) pairs, 2^31 positions and channels" % (tuple(x.shape), groups))
     for name, p in (('weight', weight), ('bias', bias)):
         if p is None:
             continue
