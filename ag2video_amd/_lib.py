@@ -158,6 +158,25 @@ def load():
     return lib
 
 
+_elem = None
+
+
+def elem_ops():
+    """The extension with the host side of the fp32 / bf16 / fp16 operators (csrc/elem_ops.cpp), bound to the loaded library."""
+    global _elem
+    if _elem is None:
+        lib = load()
+        try:
+            from . import _elem_ops as ext
+        except ImportError as e:
+            raise RuntimeError("ag2video_amd: the extension _elem_ops is not built or does not load (%s) -- make -C ag2video_amd/csrc" % e)
+        ext.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
+            'ag2v_embed_fwd', 'ag2v_embed_bwd_workspace_floats', 'ag2v_embed_bwd', 'ag2v_group_norm_workspace_floats', 'ag2v_group_norm_fwd',
+            'ag2v_group_norm_bwd')))
+        _elem = ext
+    return _elem
+
+
 _ERR = {-1: 'AG2V_EINVAL (rejected argument)', -2: 'AG2V_EHIP (HIP launch error)'}
 
 

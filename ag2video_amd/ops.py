@@ -2322,82 +2322,6 @@ def embedding(idx, table):
 
 
 # ------------------------------------------------------------------------------------------------ fp32 / bf16 / fp16 operators
-_ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_INT_LIMIT = 1 << 31
-_WS_FLOATS = {}          # workspace query and its arguments -> floats (the sizes alone decide)
-
-
-def _elem_chk(name, t):
-    if not t.is_cuda:
-        raise RuntimeError("%s: expected a HIP device tensor, got %s (no CPU fallback)" % (name, t.device))
-    if t.dtype not in _ELEM:
-        raise RuntimeError("%s: expected float32, bfloat16 or float16, got %s" % (name, t.dtype))
-
-
-def _device_guard(t):
-    """The device of ``t`` for the duration of a launch: kernels go to the current stream of the tensors' device, whichever is current."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _workspace(t, query, *args):
-    n = _WS_FLOATS.get((query, args))
-    if n is None:
-        n = _WS_FLOATS[(query, args)] = int(_lib.query(query, *args))
-    return (torch.empty(n, device=t.device, dtype=torch.float32) if n else None), n
-
-
-def _token_rows(idx):
-    """(tensor, stride): the tokens of ``idx`` in row-major order, ``stride`` elements apart; a copy only if no one stride walks them."""
-    if idx.is_contiguous():
-        return idx, 1
-    stride, run = None, 1
-    for size, st in zip(reversed(idx.shape), reversed(idx.stride())):
-        if size == 1:
-            continue
-        if stride is None:
-            stride = st
-        elif st != stride * run:
-            return idx.contiguous(), 1
-        run *= size
-    return idx, (1 if stride is None else stride)
-
-
-def _embed_fwd(idx, table, scale):
-    n, (V, D) = idx.numel(), table.shape
-    out = torch.empty(tuple(idx.shape) + (D,), device=table.device, dtype=table.dtype)
-    if n and D:
-        tok, st = _token_rows(idx)
-        with _device_guard(table):
-            _lib.call('ag2v_embed_fwd', _ELEM[table.dtype], _ptr(tok), tok.element_size(), st, _ptr(table), table.stride(0) if V > 1 else D,
-                      _ptr(out), n, V, D, scale, _stream())
-    return out
-
-
-class _EmbeddingScaled(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, idx, table, scale, pad):
-        ctx.save_for_backward(idx)
-        ctx.cfg = (tuple(table.shape), scale, pad)
-        return _embed_fwd(idx, table, scale)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        (idx,) = ctx.saved_tensors
-        (V, D), scale, pad = ctx.cfg
-        n = idx.numel()
-        if n == 0 or D == 0:
-            return None, torch.zeros((V, D), device=dout.device, dtype=dout.dtype), None, None
-        dout, _, ds = _channel_rows(dout.unsqueeze(0))
-        dtable = torch.empty((V, D), device=dout.device, dtype=dout.dtype)
-        tok, st = _token_rows(idx)
-        with _device_guard(dout):
-            ws, nws = _workspace(dout, 'ag2v_embed_bwd_workspace_floats', _ELEM[dout.dtype], n, V, D)
-            _lib.call('ag2v_embed_bwd', _ELEM[dout.dtype], _ptr(tok), tok.element_size(), st, _ptr(dout), ds, _ptr(dtable), n, V, D, scale, pad,
-                      _ptr(ws), nws, _stream())
-        return None, dtable, None, None
-
-
 def embedding_scaled(idx, table, scale=1.0, padding_idx=None):
     """scale * table[idx]: idx int32 / int64 of any shape, table [V, D] fp32, bf16 or fp16 -> idx.shape + (D,) in the table's type (the
     product in fp32, rounded once).  The rows of the result are channels-last feature vectors: group_norm_act takes them as they are.
@@ -2406,100 +2330,7 @@ def embedding_scaled(idx, table, scale=1.0, padding_idx=None):
     the row ``padding_idx`` gets none.  The tokens are sorted, so the work is that of one pass over the gradient rows and the table,
     whatever the vocabulary.  A token outside [0, V) cannot be refused without waiting for the device: its row comes back as NaN, it adds
     to no gradient, and nothing outside the table is read."""
-    _elem_chk('embedding_scaled', table)
-    if table.dim() != 2 or table.shape[0] == 0:
-        raise RuntimeError("embedding_scaled: expected a table [V > 0, D], got %s" % (tuple(table.shape),))
-    if idx.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError("embedding_scaled: expected int32 or int64 tokens, got %s" % idx.dtype)
-    if idx.device != table.device:
-        raise RuntimeError("embedding_scaled: tokens on %s, table on %s" % (idx.device, table.device))
-    if max(idx.numel(), table.shape[0], table.shape[1]) >= _INT_LIMIT:
-        raise RuntimeError("embedding_scaled: %d tokens, table %s: at most 2^31 - 1 of each" % (idx.numel(), tuple(table.shape)))
-    scale = float(scale)
-    if padding_idx is not None and not 0 <= padding_idx < table.shape[0]:
-        raise RuntimeError("embedding_scaled: padding_idx %r outside [0, %d)" % (padding_idx, table.shape[0]))
-    if table.stride(1) != 1 and table.shape[1] > 1 or table.stride(0) < table.shape[1]:
-        table = table.contiguous()
-    if torch.is_grad_enabled() and table.requires_grad:
-        return _EmbeddingScaled.apply(idx, table, scale, -1 if padding_idx is None else int(padding_idx))
-    return _embed_fwd(idx, table, scale)
-
-
-def _channel_rows(x):
-    """(tensor, sample stride, row stride) of x [N, ..., C]: its positions ``row stride`` elements apart, channels adjacent.  Channel
-    slices, channels-last views of NCHW tensors and broadcast gradients keep their memory; other orders are copied."""
-    C = x.shape[-1]
-    if x.is_contiguous():
-        return x, x[0].numel() if x.shape[0] else 0, C
-    if C > 1 and x.stride(-1) != 1:
-        x = x.contiguous()
-        return x, x[0].numel(), C
-    row, run = None, 1
-    for size, st in zip(reversed(x.shape[1:-1]), reversed(x.stride()[1:-1])):
-        if size == 1:
-            continue
-        if row is None:
-            row = st
-        elif st != row * run:
-            x = x.contiguous()
-            return x, x[0].numel(), C
-        run *= size
-    return x, x.stride(0), (C if row is None else row)
-
-
-_ACTS = {'none': 0, 'silu': 1, 'lrelu': 2}
-
-
-def _group_norm_fwd(x, weight, bias, groups, eps, act, slope):
-    N, C = x.shape[0], x.shape[-1]
-    S = x[0].numel() // C if N else 0
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    stats = torch.empty((2, N, groups), device=x.device, dtype=torch.float32)
-    if y.numel():
-        rows, xs, xr = _channel_rows(x)
-        dt = _ELEM[x.dtype]
-        with _device_guard(x):
-            ws, nws = _workspace(x, 'ag2v_group_norm_workspace_floats', dt, N, S, C, groups, 0)
-            _lib.call('ag2v_group_norm_fwd', dt, _ptr(rows), xs, xr, _ptr(weight), _ptr(bias), _param_type(weight, bias), _ptr(y), _ptr(stats),
-                      _ptr_off(stats, N * groups), N, S, C, groups, eps, act, slope, _ptr(ws), nws, _stream())
-    return y, stats
-
-
-def _param_type(weight, bias):
-    p = weight if weight is not None else bias
-    return 0 if p is None else _ELEM[p.dtype]
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, slope):
-        y, stats = _group_norm_fwd(x, weight, bias, groups, eps, act, slope)
-        ctx.save_for_backward(x, weight, bias, stats)
-        ctx.cfg = (groups, act, slope)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        groups, act, slope = ctx.cfg
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        N, C = x.shape[0], x.shape[-1]
-        new = torch.empty if x.numel() else torch.zeros
-        dx = new(x.shape, device=x.device, dtype=x.dtype) if need_x else None
-        dw = new(C, device=x.device, dtype=weight.dtype) if need_w else None
-        db = new(C, device=x.device, dtype=bias.dtype) if need_b else None
-        if x.numel():
-            S = x[0].numel() // C
-            xr_, xs, xr = _channel_rows(x)
-            dr_, ds, dr = _channel_rows(dy)
-            dt = _ELEM[x.dtype]
-            with _device_guard(x):
-                ws, nws = _workspace(x, 'ag2v_group_norm_workspace_floats', dt, N, S, C, groups, 1)
-                _lib.call('ag2v_group_norm_bwd', dt, _ptr(dr_), ds, dr, _ptr(xr_), xs, xr, _ptr(weight), _ptr(bias), _param_type(weight, bias),
-                          _ptr(stats), _ptr_off(stats, N * groups), _ptr(dx), _ptr(dw), _ptr(db), N, S, C, groups, act, slope, _ptr(ws), nws,
-                          _stream())
-        return dx, dw, db, None, None, None, None
+    return _lib.elem_ops().embedding_scaled(idx, table, scale, padding_idx)
 
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act='silu', slope=0.2):
@@ -2510,31 +2341,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act='silu', slop
     channels are adjacent are read in place (a channel slice; ``t.permute(0, 2, 3, 1)`` of a channels-last NCHW tensor).  Gradients for x,
     weight and bias; h and the activation's derivative are computed again from x, so the tape holds x and two numbers per group.  Sums in
     fp32 in a fixed order (no atomics); y and dx of a sample do not depend on the rest of the batch."""
-    _elem_chk('group_norm_act', x)
-    if x.dim() < 2 or x.shape[-1] == 0:
-        raise RuntimeError("group_norm_act: expected x [N, ..., C > 0], got %s" % (tuple(x.shape),))
-    C, groups = x.shape[-1], int(groups)
-    if groups <= 0 or C % groups:
-        raise RuntimeError("group_norm_act: %d channels do not divide into %d groups" % (C, groups))
-    if act not in _ACTS:
-        raise RuntimeError("group_norm_act: unknown activation %r (%s)" % (act, ', '.join(sorted(_ACTS))))
-    eps, slope = float(eps), float(slope)
-    if not 0.0 <= eps < float('inf') or slope != slope:
-        raise RuntimeError("group_norm_act: eps %r, slope %r" % (eps, slope))
-    if x.shape[0] * groups >= 1 << 24 or max(x.shape[0] and x[0].numel() // C, C) >= _INT_LIMIT:
-        raise RuntimeError("group_norm_act: %s in %d groups: fewer than 2^24 (sample, group) pairs, 2^31 positions and channels" % (tuple(x.shape), groups))
-    for name, p in (('weight', weight), ('bias', bias)):
-        if p is None:
-            continue
-        if p.shape != (C,) or p.device != x.device or p.dtype not in (x.dtype, torch.float32):
-            raise RuntimeError("group_norm_act: %s must be [%d] on %s in %s or float32, got %s %s on %s" % (
-                name, C, x.device, x.dtype, tuple(p.shape), p.dtype, p.device))
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise RuntimeError("group_norm_act: weight is %s, bias %s" % (weight.dtype, bias.dtype))
-    weight, bias = _c(weight), _c(bias)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
-        return _GroupNormAct.apply(x, weight, bias, groups, eps, _ACTS[act], slope)
-    return _group_norm_fwd(x, weight, bias, groups, eps, _ACTS[act], slope)[0]
+    return _lib.elem_ops().group_norm_act(x, groups, weight, bias, eps, act, slope)
 
 
 # ------------------------------------------------------------------------------------------------ pointwise / losses

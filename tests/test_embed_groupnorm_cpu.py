@@ -94,12 +94,12 @@ def test_reference_gradients_against_differences():
 ], ids=range(11))
 def test_channel_rows(shape, view, expect):
     """Which views are read in place: (sample stride, row stride), None where the operator copies."""
-    from ag2video_amd import ops
+    from ag2video_amd import _lib
     n = 1
     for s in shape:
         n *= s
     x = view(torch.arange(float(n)).view(shape))
-    t, xs, xr = ops._channel_rows(x)
+    t, xs, xr = _lib.elem_ops().channel_rows(x)
     if expect is None:
         assert t.data_ptr() != x.data_ptr() and t.is_contiguous()
     else:
@@ -116,9 +116,9 @@ def test_channel_rows(shape, view, expect):
 @pytest.mark.parametrize("view,stride", [(lambda t: t, 1), (lambda t: t[:, :, 1], 3), (lambda t: t[::2], None), (lambda t: t[1], 1), (lambda t: t[:, 0, 0], 12),
                                          (lambda t: t.permute(2, 0, 1), None), (lambda t: t[0, 0, 0], 1), (lambda t: t[:1].expand(4, 4, 3), None)], ids=range(8))
 def test_token_rows(view, stride):
-    from ag2video_amd import ops
+    from ag2video_amd import _lib
     idx = view(torch.arange(5 * 4 * 3).view(5, 4, 3))
-    t, st = ops._token_rows(idx)
+    t, st = _lib.elem_ops().token_rows(idx)
     if stride is not None:
         assert st == stride and t.data_ptr() == idx.data_ptr()
     assert torch.equal(torch.as_strided(t, (idx.numel(),), (st,), t.storage_offset()), idx.reshape(-1))
