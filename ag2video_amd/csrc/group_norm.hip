@@ -22,7 +22,7 @@ struct GnArgs {
 
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z, float slope) {
-    if (ACT == ACT_SILU) return z * __frcp_rn(1.f + __expf(-z));
+    if (ACT == ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
     if (ACT == ACT_LRELU) return z > 0.f ? z : z * slope;
     return z;
 }
@@ -30,7 +30,7 @@ __device__ __forceinline__ float act_fwd(float z, float slope) {
 template <int ACT>
 __device__ __forceinline__ float act_bwd(float dy, float z, float slope) {
     if (ACT == ACT_SILU) {
-        const float s = __frcp_rn(1.f + __expf(-z));
+        const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
         return dy * (s * (1.f + z * (1.f - s)));
     }
     if (ACT == ACT_LRELU) return z > 0.f ? dy : dy * slope;
@@ -38,12 +38,19 @@ __device__ __forceinline__ float act_bwd(float dy, float z, float slope) {
 }
 
 // ---------------------------------------------------------------- layout shared by the kernels
-// A slab of channels (whole groups, or a tile of all channels) is walked as rows of 16-byte vectors: vector `col` of a row, `nv` of its
-// elements inside the slab.  Per-thread sums meet in LDS as rows[slot][width]; group g's share is columns [g * wg, (g + 1) * wg) of every
-// slot.  A vector lies inside one group where Cg is a multiple of the vector (then one value a thread, wg = vectors a group); elsewhere it
-// may span groups, and a thread hands over one value per channel (wg = Cg).
+// Channels are walked as rows of 16-byte vectors.  `cols` vectors side by side -- a power of two, the ones beyond the slab or tile idle --
+// and threads / cols rows at a time: thread t works on vector t % cols of row t / cols, t / cols + rows at a time, ...  Lanes of one wave
+// that hold the same vector then meet by shuffles, and what a wave (or, with more than 64 vectors, a row of threads) is left with by LDS:
+// rows[slot][cols * per], `slots` of them.
 //
-// out[g] = sum of group g's share: 2^llg lanes a group, `threads` lanes in all.
+// x_j += the same x_j of the other lanes of the wave that hold the same vector
+template <int K>
+__device__ __forceinline__ void same_vector_sums(float (&x)[K], int cols) {
+    for (int o = 32; o >= cols; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) x[k] += __shfl_xor(x[k], o, 64);
+}
+// out[g] = sum over the slots of group g's columns [g * wg, (g + 1) * wg): 2^llg lanes a group, `threads` lanes in all
 __device__ __forceinline__ void share_sums(const float* rows, int slots, int width, int wg, int ng, int llg, int t, int threads, float* out) {
     const int l = t & ((1 << llg) - 1), step = 1 << llg;
     const int dr = step / wg, dc = step - dr * wg;
@@ -60,18 +67,24 @@ __device__ __forceinline__ void share_sums(const float* rows, int slots, int wid
         if (l == 0) out[g] = s;
     }
 }
-// lanes a group in share_sums: a power of two, at most a wave
+// log2 of the lanes a group gets of `threads`: at most a wave
 static int share_lanes(int threads, int ng) {
     int l = 0;
     while (l < 6 && (2 << l) * ng <= threads) ++l;
     return l;
 }
+static int log2_up(long long v) {
+    int l = 0;
+    while ((1LL << l) < v) ++l;
+    return l;
+}
 
 // ---------------------------------------------------------------- one launch: a slab's values stay in registers
-// T threads own all S positions of kg adjacent groups of one sample: U vectors a thread, read once.  Mean, then the squared deviations
-// from it, then the result.  blockDim / T slabs a workgroup.
+// T threads own all S positions of kg adjacent groups of one sample, U vectors a thread, read once: mean, then the squared deviations from
+// it, then the result.  blockDim / T slabs a workgroup.  ONE: a thread's vector touches one group (Cg a multiple of the vector, or kg = 1);
+// otherwise sums and statistics are per channel.
 struct GnSlab {
-    int T, kg, nsets, CVw, RS, llg;   // threads, groups, sets of groups a sample, vectors a row, rows at a time, log2 of lanes a group
+    int T, kg, nsets, lc, rows, slots, wg, llg;   // threads, groups, sets of groups a sample, log2 of vectors a row, rows at a time, LDS slots and columns a group, log2 of lanes a group
     long long nslab;
 };
 
@@ -80,24 +93,42 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
     extern __shared__ float shm[];
     constexpr int V = E::V, NG = ONE ? 1 : V;        // groups a vector may touch
     const int sub = threadIdx.x / p.T, t = threadIdx.x - sub * p.T, subs = blockDim.x / p.T;
-    const int width = ONE ? p.CVw : p.CVw * V, wg = ONE ? p.CVw / p.kg : a.Cg;
-    float* rows = shm + sub * (p.RS * width + 2 * p.kg);
-    float* stat = rows + p.RS * width;
+    const int cols = 1 << p.lc, width = cols * NG;
+    float* rows = shm + sub * (p.slots * width + 2 * p.kg);
+    float* stat = rows + p.slots * width;
     const long long slab = (long long)xcd_remap(blockIdx.x, gridDim.x) * subs + sub;
     const bool live = slab < p.nslab;
     const int n = live ? (int)(slab / p.nsets) : 0, g0 = live ? (int)(slab - (long long)n * p.nsets) * p.kg : 0;
     const int ng = min(p.kg, a.G - g0), c0 = g0 * a.Cg, W = ng * a.Cg;
-    const int rs = t / p.CVw, col = t - rs * p.CVw, nv = min(V, W - col * V);
-    const bool on = live && rs < p.RS && nv > 0;
+    const int rs = t >> p.lc, col = t & (cols - 1), nv = min(V, W - col * V);
+    const bool on = live && nv > 0;
     const float inv = 1.f / ((float)a.S * (float)a.Cg);
     const typename E::T* x = (const typename E::T*)a.x + n * a.xs + c0 + col * V;
     u32x4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int r = rs + u * p.RS;
+        const int r = rs + u * p.rows;
         raw[u] = u32x4{0, 0, 0, 0};
         if (on && r < a.S) raw[u] = load_vec<E>(x + r * a.xr, nv);
     }
+    // per-thread sums to rows[slot][...]
+    const auto hand_over = [&](const float (&acc)[V]) {
+        float s[NG];
+        if (ONE) {
+            s[0] = 0.f;
+#pragma unroll
+            for (int k = 0; k < V; ++k) s[0] += acc[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < NG; ++k) s[k] = acc[k];
+        }
+        same_vector_sums(s, cols);
+        if (cols > 64 || (t & 63) < cols) {
+            const int slot = cols > 64 ? rs : t >> 6;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) rows[slot * width + col * NG + k] = s[k];
+        }
+    };
     float acc[V] = {};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -106,52 +137,45 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
 #pragma unroll
         for (int k = 0; k < V; ++k) acc[k] += v[k];
     }
-    auto hand_over = [&]() {
-        if (!on) return;
-        if (ONE) {
-            float s = 0.f;
-#pragma unroll
-            for (int k = 0; k < V; ++k) s += acc[k];
-            rows[rs * width + col] = s;
-        } else {
-#pragma unroll
-            for (int k = 0; k < V; ++k) rows[rs * width + col * V + k] = acc[k];
-        }
-    };
-    hand_over();
+    hand_over(acc);
     __syncthreads();
-    if (live) share_sums(rows, p.RS, width, wg, ng, p.llg, t, p.T, stat);
+    if (live) share_sums(rows, p.slots, width, p.wg, ng, p.llg, t, p.T, stat);
     __syncthreads();
     float mean[NG];
     int gi[NG];
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-        gi[k] = min(ONE ? col / wg : (col * V + k) / a.Cg, ng - 1);
+        gi[k] = min(ONE ? col / p.wg : (col * V + k) / a.Cg, ng - 1);
         mean[k] = on ? stat[gi[k]] * inv : 0.f;
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) acc[k] = 0.f;
+    if (on) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (rs + u * p.RS < a.S) {
-            float v[V];
-            E::unpack(raw[u], v);
+        for (int u = 0; u < U; ++u)
+            if (rs + u * p.rows < a.S) {
+                float v[V];
+                E::unpack(raw[u], v);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float d = v[k] - mean[k % NG];
-                acc[k] = fmaf(d, d, acc[k]);
+                for (int k = 0; k < V; ++k) {
+                    const float d = v[k] - mean[k % NG];
+                    acc[k] = fmaf(d, d, acc[k]);
+                }
             }
+    }
+    if (nv < V) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = k < nv ? acc[k] : 0.f;
+    }
+    hand_over(acc);
+    __syncthreads();
+    if (live) share_sums(rows, p.slots, width, p.wg, ng, p.llg, t, p.T, stat + p.kg);
+    __syncthreads();
+    if (live)
+        for (int g = t; g < ng; g += p.T) {
+            a.mean[n * a.G + g0 + g] = stat[g] * inv;
+            a.rstd[n * a.G + g0 + g] = 1.f / sqrtf(stat[p.kg + g] * inv + a.eps);
         }
-    }
-    __syncthreads();
-    hand_over();
-    __syncthreads();
-    if (live) share_sums(rows, p.RS, width, wg, ng, p.llg, t, p.T, stat + p.kg);
-    __syncthreads();
-    if (live && t < ng) {
-        a.mean[n * a.G + g0 + t] = stat[t] * inv;
-        a.rstd[n * a.G + g0 + t] = 1.f / sqrtf(stat[p.kg + t] * inv + a.eps);
-    }
     if (!on) return;
     float w[V], b[V], rstd[NG];
 #pragma unroll
@@ -165,7 +189,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
     typename E::T* y = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + col * V;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int r = rs + u * p.RS;
+        const int r = rs + u * p.rows;
         if (r < a.S) {
             float v[V];
             E::unpack(raw[u], v);
@@ -177,32 +201,34 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
 }
 
 // Backward on slabs: x and dy of a slab in registers.  A workgroup keeps its set of groups and walks samples, `walkers` apart, so that the
-// parameters' gradients leave it once: ab[walker][C] = (sum dz, sum dz h) over its samples.  Vectors that span groups hold statistics per
-// channel and half as many rows (512 threads, 256 registers each).
+// parameters' gradients leave it once: ab[walker][C] = (sum dz, sum dz h) over its samples.  Without ONE the statistics are per channel and
+// take 512 threads of 256 registers.
 template <class E, int ACT, int U, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a, GnSlab p, int walkers, float2* ab) {
     extern __shared__ float shm[];
     constexpr int V = E::V, NG = ONE ? 1 : V;
     const int sub = threadIdx.x / p.T, t = threadIdx.x - sub * p.T, subs = blockDim.x / p.T;
-    const int width = p.CVw * V, swidth = ONE ? p.CVw : width, wg = ONE ? p.CVw / p.kg : a.Cg;
-    const int area = p.RS * (ONE ? width : 2 * width);           // two arrays of group sums while walking, one of channel sums at the end
+    const int cols = 1 << p.lc, width = cols * V, gwidth = cols * NG;
+    // two arrays of group sums while walking, one of channel sums at the end
+    const int area = p.slots * (ONE ? width : 2 * width);
     float* r1 = shm + sub * (area + 2 * p.kg);
-    float* r2 = r1 + p.RS * swidth;
+    float* r2 = r1 + p.slots * gwidth;
     float* stat = r1 + area;
     const int blk = xcd_remap(blockIdx.x, gridDim.x), set = blk % p.nsets, walker = blk / p.nsets * subs + sub;
     const int g0 = set * p.kg, ng = min(p.kg, a.G - g0), c0 = g0 * a.Cg, W = ng * a.Cg;
-    const int rs = t / p.CVw, col = t - rs * p.CVw, nv = min(V, W - col * V);
-    const bool on = rs < p.RS && nv > 0;
+    const int rs = t >> p.lc, col = t & (cols - 1), nv = min(V, W - col * V);
+    const bool on = nv > 0, writes = cols > 64 || (t & 63) < cols;
+    const int slot = cols > 64 ? rs : t >> 6;
     const float inv = 1.f / ((float)a.S * (float)a.Cg);
     float w[V], b[V], A[V], B[V];
     int gi[NG];
 #pragma unroll
-    for (int k = 0; k < NG; ++k) gi[k] = min(ONE ? col / wg : (col * V + k) / a.Cg, ng - 1);
+    for (int k = 0; k < NG; ++k) gi[k] = min(ONE ? col / p.wg : (col * V + k) / a.Cg, ng - 1);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         const int c = c0 + col * V + k;
-        w[k] = a.w && on && k < nv ? load_any(a.w, a.ptype, c) : 1.f;
-        b[k] = a.b && on && k < nv ? load_any(a.b, a.ptype, c) : 0.f;
+        w[k] = a.w && k < nv ? load_any(a.w, a.ptype, c) : 1.f;
+        b[k] = a.b && k < nv ? load_any(a.b, a.ptype, c) : 0.f;
         A[k] = B[k] = 0.f;
     }
     for (int n0 = blk / p.nsets * subs; n0 < a.N; n0 += walkers) {
@@ -213,49 +239,58 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
         const typename E::T* dy = (const typename E::T*)a.dy + (long long)n * a.ds + c0 + col * V;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = rs + u * p.RS;
+            const int r = rs + u * p.rows;
             rx[u] = rd[u] = u32x4{0, 0, 0, 0};
             if (here && r < a.S) {
                 rx[u] = load_vec<E>(x + r * a.xr, nv);
                 rd[u] = load_vec<E>(dy + r * a.dr, nv);
             }
         }
-        float mean[NG], rstd[NG], g1[NG] = {}, g2[NG] = {};     // g1, g2: sums of w dz and w dz h
+        float off[NG], rstd[NG], g1[NG] = {}, g2[NG] = {};      // h = x rstd + off; g1, g2: sums of w dz and w dz h
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
-            mean[k] = here ? a.mean[(long long)n * a.G + g0 + gi[k]] : 0.f;
             rstd[k] = here ? a.rstd[(long long)n * a.G + g0 + gi[k]] : 0.f;
+            off[k] = here ? -a.mean[(long long)n * a.G + g0 + gi[k]] * rstd[k] : 0.f;
         }
         if (here) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (rs + u * p.RS < a.S) {
+                if (rs + u * p.rows < a.S) {
                     float v[V], d[V];
                     E::unpack(rx[u], v);
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = (v[k] - mean[k % NG]) * rstd[k % NG], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope), e = w[k] * dz;
+                        const float h = fmaf(v[k], rstd[k % NG], off[k % NG]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope), e = w[k] * dz;
                         A[k] += dz;
                         B[k] = fmaf(dz, h, B[k]);
                         g1[k % NG] += e;
                         g2[k % NG] = fmaf(e, h, g2[k % NG]);
                     }
                 }
+        }
+        if (a.y) {
+            same_vector_sums(g1, cols);
+            same_vector_sums(g2, cols);
+            if (writes) {
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                r1[rs * swidth + (ONE ? col : col * V + k)] = g1[k];
-                r2[rs * swidth + (ONE ? col : col * V + k)] = g2[k];
+                for (int k = 0; k < NG; ++k) {
+                    r1[slot * gwidth + col * NG + k] = g1[k];
+                    r2[slot * gwidth + col * NG + k] = g2[k];
+                }
             }
+            __syncthreads();
+            if (live) {
+                share_sums(r1, p.slots, gwidth, p.wg, ng, p.llg, t, p.T, stat);
+                share_sums(r2, p.slots, gwidth, p.wg, ng, p.llg, t, p.T, stat + p.kg);
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        if (live && a.y) {
-            share_sums(r1, p.RS, swidth, wg, ng, p.llg, t, p.T, stat);
-            share_sums(r2, p.RS, swidth, wg, ng, p.llg, t, p.T, stat + p.kg);
-        }
-        __syncthreads();
         if (here && a.y) {
             typename E::T* dx = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + col * V;
+            // (the values above are computed again: kept, they would not fit the registers)
+#pragma unroll
+            for (int u = 0; u < U; ++u) asm volatile("" : "+v"(rx[u]), "+v"(rd[u]));
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
                 g1[k] = stat[gi[k]] * inv;
@@ -263,14 +298,14 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int r = rs + u * p.RS;
+                const int r = rs + u * p.rows;
                 if (r < a.S) {
                     float v[V], d[V];
                     E::unpack(rx[u], v);
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = (v[k] - mean[k % NG]) * rstd[k % NG], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                        const float h = fmaf(v[k], rstd[k % NG], off[k % NG]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                         v[k] = rstd[k % NG] * (w[k] * dz - g1[k % NG] - h * g2[k % NG]);
                     }
                     store_vec<E>(dx + (long long)r * a.C, nv, v);
@@ -280,156 +315,175 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
     }
     if (!ab) return;
     // the channels' sums over the workgroup's rows, one array at a time in all of the rows' memory
+    same_vector_sums(A, cols);
+    same_vector_sums(B, cols);
     for (int half = 0; half < 2; ++half) {
         __syncthreads();
-        if (on) {
+        if (writes) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) r1[rs * width + col * V + k] = half ? B[k] : A[k];
+            for (int k = 0; k < V; ++k) r1[slot * width + col * V + k] = half ? B[k] : A[k];
         }
         __syncthreads();
         for (int c = t; c < W; c += p.T) {
             float s = 0.f;
-            for (int r = 0; r < p.RS; ++r) s += r1[r * width + c];
+            for (int r = 0; r < p.slots; ++r) s += r1[r * width + c];
             (&ab[(long long)walker * a.C + c0 + c].x)[half] = s;
         }
     }
 }
 
 // ---------------------------------------------------------------- larger maps: sums of parts, a join, a second pass over the map
-// A workgroup owns `rows` positions of one sample and a tile of CVt vectors of channels.
+// A workgroup owns `len` positions of one sample and a tile of 2^lc vectors of channels.
 struct GnParts {
-    int tiles, CVt, RS, rows, P, llg;    // P: parts a sample
+    int tiles, lc, rows, slots, len, P, tg, llg;    // P: parts a sample; tg: tiles a group may touch
 };
+struct GnWhere {
+    int tile, n, q, rs, col, c0, W, nv, lo, hi;
+};
+template <int V>
+__device__ __forceinline__ GnWhere where_of(const GnArgs& a, const GnParts& p, int blk) {
+    GnWhere i;
+    i.tile = blk % p.tiles;
+    const int np = blk / p.tiles;
+    i.n = np / p.P;
+    i.q = np - i.n * p.P;
+    i.rs = threadIdx.x >> p.lc;
+    i.col = threadIdx.x & ((1 << p.lc) - 1);
+    i.c0 = (i.tile * V) << p.lc;
+    i.W = min(V << p.lc, a.C - i.c0);
+    i.nv = min(V, i.W - i.col * V);
+    i.lo = i.q * p.len;
+    i.hi = min(a.S, i.lo + p.len);
+    return i;
+}
 
-// Every thread sums deviations from the first value it sees of each channel.  That value is one of the summed ones, so the sum of squares
-// about it is at most (count + 1) times the one about the thread's mean: nothing cancels that matters, whatever the mean is.
-// part[n][p * tiles + tile][g] = (count, mean, sum of squares about it)
+// Statistics of a part.  A thread sums deviations from the first value it sees of each channel: that value is one of the summed ones, so the
+// sum of squares about it is at most (count + 1) times the one about the thread's mean, and nothing cancels that matters, whatever the mean.
+// Threads, waves and channels then join pairwise as (count, mean, squares about the mean).
+// part[n][g][q * tg + (tile - the group's first tile)] = (count, mean, squares, 0)
 template <class E>
-__global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, float* part) {
-    __shared__ float r1[256 * E::V], r2[256 * E::V];
-    __shared__ float gs[2][256];
+__global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, float4* part) {
     constexpr int V = E::V, U = 8;
-    const int tile = blockIdx.x % p.tiles, np = blockIdx.x / p.tiles, n = np / p.P, q = np - n * p.P;
-    const int rs = threadIdx.x / p.CVt, col = threadIdx.x - rs * p.CVt, c0 = tile * p.CVt * V, W = min(p.CVt * V, a.C - c0);
-    const int nv = min(V, W - col * V);
-    const bool on = rs < p.RS && nv > 0;
-    const int lo = q * p.rows, hi = min(a.S, lo + p.rows);
-    const typename E::T* x = (const typename E::T*)a.x + n * a.xs + c0 + col * V;
-    float x0[V] = {}, s[V] = {}, m[V] = {};
-    int cnt = 0;
-    if (on && lo + rs < hi) {
-        E::unpack(load_vec<E>(x + (lo + rs) * a.xr, nv), x0);
-        for (int r = lo + rs; r < hi; r += U * p.RS) {
+    __shared__ float sm[4 * 64 * V], sq[4 * 64 * V], sn[4];      // [slot][width]
+    const GnWhere i = where_of<V>(a, p, blockIdx.x);
+    const int cols = 1 << p.lc, width = cols * V;
+    const bool on = i.nv > 0;
+    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c0 + i.col * V;
+    float mean[V] = {}, s[V] = {}, m[V] = {};
+    int count = 0;
+    if (on && i.lo + i.rs < i.hi) {
+        for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
             u32x4 raw[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r + u * p.RS < hi) raw[u] = load_vec<E>(x + (long long)(r + u * p.RS) * a.xr, nv);
+                if (r + u * p.rows < i.hi) raw[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
+            if (count == 0) E::unpack(raw[0], mean);
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r + u * p.RS < hi) {
+                if (r + u * p.rows < i.hi) {
                     float v[V];
                     E::unpack(raw[u], v);
-                    ++cnt;
+                    ++count;
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float d = v[k] - x0[k];
+                        const float d = v[k] - mean[k];
                         s[k] += d;
                         m[k] = fmaf(d, d, m[k]);
                     }
                 }
         }
-    }
-    // per channel and slot: mean and squares about it; then the groups' means, then the squares about those
-    const int width = p.CVt * V;
-    float mean[V];
+        const float rc = 1.f / (float)count;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const float ds = cnt ? s[k] / (float)cnt : 0.f;
-        mean[k] = x0[k] + ds;
-        const float m2 = m[k] - s[k] * ds;
-        m[k] = m2 < 0.f ? 0.f : m2;
-        if (on) r1[rs * width + col * V + k] = mean[k] * (float)cnt;
+        for (int k = 0; k < V; ++k) {
+            const float ds = s[k] * rc, q = fmaf(-s[k], ds, m[k]);
+            mean[k] += ds;
+            m[k] = q < 0.f ? 0.f : q;
+        }
+    }
+    // lanes with the same vector
+    float nn = (float)max(0, (i.hi - i.lo - i.rs + p.rows - 1) / p.rows);
+    for (int o = 32; o >= cols; o >>= 1) {
+        const float nb = __shfl_xor(nn, o, 64), nt = nn + nb, f = nt > 0.f ? nb / nt : 0.f, nf = nn * f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float mb = __shfl_xor(mean[k], o, 64), qb = __shfl_xor(m[k], o, 64), d = nt > nn ? mb - mean[k] : 0.f;
+            mean[k] = nn > 0.f ? fmaf(d, f, mean[k]) : mb;
+            m[k] += qb + d * d * nf;
+        }
+        nn = nt;
+    }
+    const int slot = cols > 64 ? i.rs : threadIdx.x >> 6;
+    if (cols > 64 || (threadIdx.x & 63) < cols) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            sm[slot * width + i.col * V + k] = mean[k];
+            sq[slot * width + i.col * V + k] = m[k];
+        }
+        if (i.col == 0) sn[slot] = nn;
     }
     __syncthreads();
-    // groups whose channels lie (partly) in this tile
-    const int gl = c0 / a.Cg, gh = (c0 + W - 1) / a.Cg;
-    for (int g0 = gl; g0 <= gh; g0 += 256) {
-        const int ng = min(256, gh - g0 + 1);
-        // lanes a group: all threads shared over the groups, a power of two within a wave
-        const int llg = p.llg, step = 1 << llg, l = threadIdx.x & (step - 1);
-        for (int round = 0; round < 2; ++round) {
-            for (int g = threadIdx.x >> llg; g < ng; g += 256 >> llg) {
-                const int cl = max((g0 + g) * a.Cg - c0, 0), wg = min((g0 + g + 1) * a.Cg - c0, W) - cl;
-                float t = 0.f;
-                for (int e = l; e < p.RS * wg; e += step) {
-                    const int r = e / wg, c = e - r * wg;
-                    t += (round ? r2 : r1)[r * width + cl + c];
-                }
-                for (int o = step >> 1; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-                if (l == 0) gs[round][g] = t;
-            }
-            __syncthreads();
-            if (round == 0) {
-                const int slots = min(p.RS, hi - lo);
-                const float rows = (float)(hi - lo);
-                if (on && rs < slots) {
-#pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        const int g = (c0 + col * V + k) / a.Cg - g0;
-                        if (k < nv && g >= 0 && g < ng) {
-                            const int cl = max((g0 + g) * a.Cg - c0, 0), wg = min((g0 + g + 1) * a.Cg - c0, W) - cl;
-                            const float d = mean[k] - gs[0][g] / (rows * (float)wg);
-                            r2[rs * width + col * V + k] = fmaf(d * d, (float)cnt, m[k]);
-                        }
-                    }
-                } else if (on) {
-#pragma unroll
-                    for (int k = 0; k < V; ++k) r2[rs * width + col * V + k] = 0.f;
-                }
-                __syncthreads();
+    // the slots of a channel, to slot 0
+    const float rows = (float)(i.hi - i.lo);
+    for (int c = threadIdx.x; c < i.W; c += 256) {
+        float n = sn[0], mc = sm[c], qc = sq[c];
+        for (int w = 1; w < p.slots; ++w) {
+            const float nb = sn[w], d = sm[w * width + c] - mc, nt = n + nb;
+            if (nb > 0.f) {
+                mc = fmaf(d, nb / nt, mc);
+                qc += sq[w * width + c] + d * d * (n * nb / nt);
+                n = nt;
             }
         }
-        for (int g = threadIdx.x; g < ng; g += 256) {
-            const int cl = max((g0 + g) * a.Cg - c0, 0), wg = min((g0 + g + 1) * a.Cg - c0, W) - cl;
-            const float count = (float)(hi - lo) * (float)wg;
-            float* o = part + (((long long)n * p.P + q) * p.tiles + tile) * a.G * 3 + (long long)(g0 + g) * 3;
-            o[0] = count;
-            o[1] = gs[0][g] / count;
-            o[2] = gs[1][g];
-        }
-        __syncthreads();
+        sm[c] = mc;
+        sq[c] = qc;
     }
-    for (int g = threadIdx.x; g < a.G; g += 256)
-        if (g < gl || g > gh) part[((((long long)n * p.P + q) * p.tiles + tile) * a.G + g) * 3] = 0.f;
+    __syncthreads();
+    // the channels of a group: 2^llg lanes each
+    const int gl = i.c0 / a.Cg, gh = (i.c0 + i.W - 1) / a.Cg, step = 1 << p.llg, l = threadIdx.x & (step - 1);
+    for (int g = gl + (threadIdx.x >> p.llg); g <= gh; g += 256 >> p.llg) {
+        const int cl = max(g * a.Cg - i.c0, 0), ch = min((g + 1) * a.Cg - i.c0, i.W);
+        float t = 0.f, q = 0.f;
+        for (int c = cl + l; c < ch; c += step) t += sm[c];
+        for (int o = step >> 1; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+        const float gm = t / (float)(ch - cl);
+        for (int c = cl + l; c < ch; c += step) {
+            const float d = sm[c] - gm;
+            q += sq[c] + rows * (d * d);
+        }
+        for (int o = step >> 1; o > 0; o >>= 1) q += __shfl_xor(q, o, 64);
+        if (l == 0)
+            part[((long long)i.n * a.G + g) * p.P * p.tg + i.q * p.tg + i.tile - g * a.Cg / (V << p.lc)] = make_float4(rows * (float)(ch - cl), gm, q, 0.f);
+    }
 }
 
-// A wave per (sample, group): the parts' means and squares joined pairwise, in fp64.
-__global__ __launch_bounds__(256) void gn_stats_join_kernel(GnArgs a, int parts, const float* part) {
-    const int ngroups = a.N * a.G, id = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
-    if (id >= ngroups) return;
-    const int n = id / a.G, g = id - n * a.G;
+// A wave per (sample, group): its parts joined pairwise, in fp64.
+template <int V>
+__global__ __launch_bounds__(256) void gn_stats_join_kernel(GnArgs a, GnParts p, const float4* part) {
+    const int id = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
+    if (id >= a.N * a.G) return;
+    const int g = id % a.G, tw = V << p.lc, tg = ((g + 1) * a.Cg - 1) / tw - g * a.Cg / tw + 1;    // tiles the group touches
     double cnt = 0.0, mean = 0.0, m2 = 0.0;
-    auto join = [&](double cb, double mb, double qb) {
+    const auto join = [&](double cb, double mb, double qb) {
         if (cb == 0.0) return;
-        const double c = cnt + cb, d = mb - mean;
-        mean += d * (cb / c);
-        m2 += qb + d * d * (cnt * cb / c);
+        const double c = cnt + cb, d = mb - mean, f = cb / c;
+        mean += d * f;
+        m2 += qb + d * d * (cnt * f);
         cnt = c;
     };
-    for (int i = l; i < parts; i += 64) {
-        const float* o = part + (((long long)n * parts + i) * a.G + g) * 3;
-        join(o[0], o[1], o[2]);
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-        const double cb = __shfl_xor(cnt, o, 64), mb = __shfl_xor(mean, o, 64), qb = __shfl_xor(m2, o, 64);
-        // both partners form the same pair in the same order
-        if (l & o) {
-            const double c1 = cnt, m1 = mean, q1 = m2;
-            cnt = cb; mean = mb; m2 = qb;
-            join(c1, m1, q1);
-        } else {
-            join(cb, mb, qb);
+    const float4* mine = part + (long long)id * p.P * p.tg;
+    for (int i = l; i < p.P * p.tg; i += 64)
+        if (i % p.tg < tg) {
+            const float4 o = mine[i];
+            join(o.x, o.y, o.z);
         }
+    for (int o = 32; o > 0; o >>= 1) {
+        double cb = __shfl_xor(cnt, o, 64), mb = __shfl_xor(mean, o, 64), qb = __shfl_xor(m2, o, 64);
+        if (l & o) {          // both partners form the same pair in the same order
+            const double c = cnt, m = mean, q = m2;
+            cnt = cb; mean = mb; m2 = qb;
+            cb = c; mb = m; qb = q;
+        }
+        join(cb, mb, qb);
     }
     if (l == 0) {
         a.mean[id] = (float)mean;
@@ -440,104 +494,96 @@ __global__ __launch_bounds__(256) void gn_stats_join_kernel(GnArgs a, int parts,
 template <class E, int ACT>
 __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p) {
     constexpr int V = E::V, U = 4;
-    const int tile = blockIdx.x % p.tiles, np = blockIdx.x / p.tiles, n = np / p.P, q = np - n * p.P;
-    const int rs = threadIdx.x / p.CVt, col = threadIdx.x - rs * p.CVt, c0 = tile * p.CVt * V, W = min(p.CVt * V, a.C - c0);
-    const int nv = min(V, W - col * V), lo = q * p.rows, hi = min(a.S, lo + p.rows);
-    if (rs >= p.RS || nv <= 0) return;
+    const GnWhere i = where_of<V>(a, p, blockIdx.x);
+    if (i.nv <= 0) return;
     float mean[V], w[V], b[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int c = min(c0 + col * V + k, a.C - 1), g = n * a.G + c / a.Cg;
+        const int c = min(i.c0 + i.col * V + k, a.C - 1), g = i.n * a.G + c / a.Cg;
         mean[k] = a.mean[g];
         w[k] = (a.w ? load_any(a.w, a.ptype, c) : 1.f) * a.rstd[g];
         b[k] = a.b ? load_any(a.b, a.ptype, c) : 0.f;
     }
-    const typename E::T* x = (const typename E::T*)a.x + n * a.xs + c0 + col * V;
-    typename E::T* y = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + col * V;
-    for (int r = lo + rs; r < hi; r += U * p.RS) {
+    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c0 + i.col * V;
+    typename E::T* y = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c0 + i.col * V;
+    for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
         u32x4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (r + u * p.RS < hi) raw[u] = load_vec<E>(x + (long long)(r + u * p.RS) * a.xr, nv);
+            if (r + u * p.rows < i.hi) raw[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (r + u * p.RS < hi) {
+            if (r + u * p.rows < i.hi) {
                 float v[V];
                 E::unpack(raw[u], v);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[k] = act_fwd<ACT>(fmaf(v[k] - mean[k], w[k], b[k]), a.slope);
-                store_vec<E>(y + (long long)(r + u * p.RS) * a.C, nv, v);
+                store_vec<E>(y + (long long)(r + u * p.rows) * a.C, i.nv, v);
             }
     }
 }
 
-// part[n][p][c] = (sum dz, sum dz h) over the part's positions
+// part[n][q][c] = (sum dz, sum dz h) over the part's positions
 template <class E, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, float2* part) {
-    __shared__ float r1[256 * E::V], r2[256 * E::V];
     constexpr int V = E::V, U = 4;
-    const int tile = blockIdx.x % p.tiles, np = blockIdx.x / p.tiles, n = np / p.P, q = np - n * p.P;
-    const int rs = threadIdx.x / p.CVt, col = threadIdx.x - rs * p.CVt, c0 = tile * p.CVt * V, W = min(p.CVt * V, a.C - c0);
-    const int nv = min(V, W - col * V), lo = q * p.rows, hi = min(a.S, lo + p.rows);
-    const bool on = rs < p.RS && nv > 0;
+    __shared__ float r1[4 * 64 * V], r2[4 * 64 * V];
+    const GnWhere i = where_of<V>(a, p, blockIdx.x);
+    const int cols = 1 << p.lc, width = cols * V;
     float A[V] = {}, B[V] = {};
-    if (on) {
-        float mean[V], rstd[V], w[V], b[V];
+    if (i.nv > 0) {
+        float off[V], rstd[V], w[V], b[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const int c = min(c0 + col * V + k, a.C - 1), g = n * a.G + c / a.Cg;
-            mean[k] = a.mean[g];
+            const int c = min(i.c0 + i.col * V + k, a.C - 1), g = i.n * a.G + c / a.Cg;
             rstd[k] = a.rstd[g];
+            off[k] = -a.mean[g] * rstd[k];
             w[k] = a.w ? load_any(a.w, a.ptype, c) : 1.f;
             b[k] = a.b ? load_any(a.b, a.ptype, c) : 0.f;
         }
-        const typename E::T* x = (const typename E::T*)a.x + n * a.xs + c0 + col * V;
-        const typename E::T* dy = (const typename E::T*)a.dy + n * a.ds + c0 + col * V;
-        for (int r = lo + rs; r < hi; r += U * p.RS) {
+        const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c0 + i.col * V;
+        const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c0 + i.col * V;
+        for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
             u32x4 rx[U], rd[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r + u * p.RS < hi) {
-                    rx[u] = load_vec<E>(x + (long long)(r + u * p.RS) * a.xr, nv);
-                    rd[u] = load_vec<E>(dy + (long long)(r + u * p.RS) * a.dr, nv);
+                if (r + u * p.rows < i.hi) {
+                    rx[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
+                    rd[u] = load_vec<E>(dy + (long long)(r + u * p.rows) * a.dr, i.nv);
                 }
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r + u * p.RS < hi) {
+                if (r + u * p.rows < i.hi) {
                     float v[V], d[V];
                     E::unpack(rx[u], v);
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = (v[k] - mean[k]) * rstd[k], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                        const float h = fmaf(v[k], rstd[k], off[k]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                         A[k] += dz;
                         B[k] = fmaf(dz, h, B[k]);
                     }
                 }
         }
     }
-    const int width = p.CVt * V;
-    if (on) {
+    same_vector_sums(A, cols);
+    same_vector_sums(B, cols);
+    if (cols > 64 || (threadIdx.x & 63) < cols) {
+        const int slot = cols > 64 ? i.rs : threadIdx.x >> 6;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            r1[rs * width + col * V + k] = A[k];
-            r2[rs * width + col * V + k] = B[k];
+            r1[slot * width + i.col * V + k] = A[k];
+            r2[slot * width + i.col * V + k] = B[k];
         }
     }
     __syncthreads();
-    // lanes share a channel's slots where channels are few
-    const int step = 1 << p.llg, l = threadIdx.x & (step - 1);
-    for (int c = threadIdx.x >> p.llg; c < W; c += 256 >> p.llg) {
+    for (int c = threadIdx.x; c < i.W; c += 256) {
         float s = 0.f, t = 0.f;
-        for (int r = l; r < p.RS; r += step) {
+        for (int r = 0; r < p.slots; ++r) {
             s += r1[r * width + c];
             t += r2[r * width + c];
         }
-        for (int o = step >> 1; o > 0; o >>= 1) {
-            s += __shfl_xor(s, o, 64);
-            t += __shfl_xor(t, o, 64);
-        }
-        if (l == 0) part[((long long)n * p.P + q) * a.C + c0 + c] = make_float2(s, t);
+        part[((long long)i.n * p.P + i.q) * a.C + i.c0 + c] = make_float2(s, t);
     }
 }
 
@@ -550,20 +596,34 @@ __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int l
     for (int c0 = 0; c0 < a.Cg; c0 += cw) {
         const int c = g * a.Cg + c0 + cl;
         float2 v = make_float2(0.f, 0.f);
-        if (c0 + cl < a.Cg)
-            for (int q = slot; q < P; q += slots) {
-                const float2 o = part[((long long)n * P + q) * a.C + c];
+        if (c0 + cl < a.Cg) {
+            const float2* mine = part + (long long)n * P * a.C + c;
+            int q = slot;
+            for (; q + 3 * slots < P; q += 4 * slots) {
+                float2 o[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) o[u] = mine[(long long)(q + u * slots) * a.C];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) { v.x += o[u].x; v.y += o[u].y; }
+            }
+            for (; q < P; q += slots) {
+                const float2 o = mine[(long long)q * a.C];
                 v.x += o.x;
                 v.y += o.y;
             }
+        }
         sh[threadIdx.x] = v;
         __syncthreads();
-        if (slot == 0 && c0 + cl < a.Cg) {
-            for (int q = 1; q < slots; ++q) {
-                const float2 o = sh[(q << lcw) + cl];
-                v.x += o.x;
-                v.y += o.y;
+        for (int o = slots >> 1; o > 0; o >>= 1) {
+            if (slot < o) {
+                const float2 q = sh[((slot + o) << lcw) + cl];
+                v.x += q.x;
+                v.y += q.y;
+                sh[threadIdx.x] = v;
             }
+            __syncthreads();
+        }
+        if (slot == 0 && c0 + cl < a.Cg) {
             ab[(long long)n * a.C + c] = v;
             const float w = a.w ? load_any(a.w, a.ptype, c) : 1.f;
             s1 = fmaf(w, v.x, s1);
@@ -586,44 +646,42 @@ __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int l
 template <class E, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef) {
     constexpr int V = E::V, U = 4;
-    const int tile = blockIdx.x % p.tiles, np = blockIdx.x / p.tiles, n = np / p.P, q = np - n * p.P;
-    const int rs = threadIdx.x / p.CVt, col = threadIdx.x - rs * p.CVt, c0 = tile * p.CVt * V, W = min(p.CVt * V, a.C - c0);
-    const int nv = min(V, W - col * V), lo = q * p.rows, hi = min(a.S, lo + p.rows);
-    if (rs >= p.RS || nv <= 0) return;
-    float mean[V], rstd[V], w[V], b[V], s1[V], s2[V];
+    const GnWhere i = where_of<V>(a, p, blockIdx.x);
+    if (i.nv <= 0) return;
+    float off[V], rstd[V], w[V], b[V], s1[V], s2[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int c = min(c0 + col * V + k, a.C - 1), g = n * a.G + c / a.Cg;
-        mean[k] = a.mean[g];
+        const int c = min(i.c0 + i.col * V + k, a.C - 1), g = i.n * a.G + c / a.Cg;
         rstd[k] = a.rstd[g];
+        off[k] = -a.mean[g] * rstd[k];
         w[k] = a.w ? load_any(a.w, a.ptype, c) : 1.f;
         b[k] = a.b ? load_any(a.b, a.ptype, c) : 0.f;
         s1[k] = coef[g].x;
         s2[k] = coef[g].y;
     }
-    const typename E::T* x = (const typename E::T*)a.x + n * a.xs + c0 + col * V;
-    const typename E::T* dy = (const typename E::T*)a.dy + n * a.ds + c0 + col * V;
-    typename E::T* dx = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + col * V;
-    for (int r = lo + rs; r < hi; r += U * p.RS) {
+    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c0 + i.col * V;
+    const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c0 + i.col * V;
+    typename E::T* dx = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c0 + i.col * V;
+    for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
         u32x4 rx[U], rd[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (r + u * p.RS < hi) {
-                rx[u] = load_vec<E>(x + (long long)(r + u * p.RS) * a.xr, nv);
-                rd[u] = load_vec<E>(dy + (long long)(r + u * p.RS) * a.dr, nv);
+            if (r + u * p.rows < i.hi) {
+                rx[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
+                rd[u] = load_vec<E>(dy + (long long)(r + u * p.rows) * a.dr, i.nv);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (r + u * p.RS < hi) {
+            if (r + u * p.rows < i.hi) {
                 float v[V], d[V];
                 E::unpack(rx[u], v);
                 E::unpack(rd[u], d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    const float h = (v[k] - mean[k]) * rstd[k], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                    const float h = fmaf(v[k], rstd[k], off[k]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                     v[k] = rstd[k] * (w[k] * dz - s1[k] - h * s2[k]);
                 }
-                store_vec<E>(dx + (long long)(r + u * p.RS) * a.C, nv, v);
+                store_vec<E>(dx + (long long)(r + u * p.rows) * a.C, i.nv, v);
             }
     }
 }
@@ -656,78 +714,92 @@ static int vec_of(int dtype) { return dtype == AG2V_F32 ? ElemF32::V : ElemBF16:
 
 // Which way (N, S, C, G) runs, forward or backward.
 struct GnPlan {
-    bool slab, one;                  // one: a vector lies inside one group
+    bool slab, one;
     GnSlab s;
     int U, threads, blocks, walkers;
     size_t lds;
     GnParts p;
     long long words, ab, coef;       // workspace in floats; offsets of ab[][C] and coef[N][G] in it
 };
+#ifndef GN_SLAB_FWD
+#define GN_SLAB_FWD 8192
+#define GN_SLAB_BWD 2048
+#endif
+static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backward) {
+    const int Cg = C / G;
+    const auto lcols = [&](int k) { return log2_up(((long long)k * Cg + V - 1) / V); };
+    const long long most = backward ? GN_SLAB_BWD : GN_SLAB_FWD;        // vectors a slab
+    // groups of a slab: rows of 128 bytes where that fits, so that slabs share no cache line
+    int kg = 1;
+    while (kg < G && (long long)kg * Cg < 8 * V && lcols(kg + 1) <= 3 && ((long long)S << lcols(kg + 1)) <= most) ++kg;
+    const int lc = lcols(kg);
+    if (lc > 10 || ((long long)S << lc) > most) return false;
+    const bool one = kg == 1 || Cg % V == 0;
+    const int maxT = backward && !one ? 512 : 1024, maxU = backward ? 2 : 8;
+    int T = 64;
+    while (T < maxT && (((long long)S << lc) > (long long)T * (maxU < 4 ? maxU : 4) || T < (1 << lc))) T *= 2;
+    if (T < (1 << lc)) return false;
+    const int rows = T >> lc, U = (S + rows - 1) / rows;
+    if (U > maxU) return false;
+    r.slab = true;
+    r.one = one;
+    r.U = U <= 1 ? 1 : U <= 2 ? 2 : U <= 4 ? 4 : 8;
+    r.threads = T < 256 ? 256 : T;
+    r.s.T = T;
+    r.s.kg = kg;
+    r.s.nsets = (G + kg - 1) / kg;
+    r.s.lc = lc;
+    r.s.rows = rows;
+    r.s.slots = lc > 6 ? rows : T / 64;
+    r.s.wg = kg == 1 && one ? 1 << lc : one ? Cg / V : Cg;
+    r.s.llg = share_lanes(T, kg);
+    r.s.nslab = (long long)N * r.s.nsets;
+    const int subs = r.threads / T;
+    r.lds = sizeof(float) * subs * (((size_t)r.s.slots << lc) * (backward ? (one ? V : 2 * V) : (one ? 1 : V)) + 2 * kg);
+    long long blocks;
+    if (!backward) {
+        blocks = (r.s.nslab + subs - 1) / subs;
+    } else {
+        long long wb = ((long long)N + subs - 1) / subs;
+        const long long cap = 2048 / r.s.nsets < 1 ? 1 : 2048 / r.s.nsets;
+        if (wb > cap) wb = cap;
+        r.walkers = (int)wb * subs;
+        blocks = wb * r.s.nsets;
+        r.words = 2LL * r.walkers * C;
+    }
+    r.blocks = (int)blocks;
+    return blocks < (1LL << 22) && r.lds <= 64 * 1024;
+}
 static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
     GnPlan r = {};
     const int V = vec_of(dtype), Cg = C / G;
-    const bool one = Cg % V == 0;
-    const int maxT = backward && !one ? 512 : 1024, maxU = !backward ? 8 : one ? 4 : 2;
-    // groups of a slab: rows of 128 bytes where that fits, so that slabs share no cache line
-    int kg = 1;
-    auto vecs = [&](int k) { return ((long long)k * Cg + V - 1) / V; };
-    while (kg < G && vecs(kg) < 128 / 16 && (long long)S * vecs(kg + 1) <= maxT * maxU) ++kg;
-    const long long cv = vecs(kg), total = (long long)S * cv;
-    if (cv <= maxT && total <= (long long)maxT * maxU) {
-        int T = 64;
-        while (T < maxT && ((long long)T * (maxU < 4 ? maxU : 4) < total || T < cv)) T *= 2;
-        const int RS = T / (int)cv;
-        const int U = (S + RS - 1) / RS;
-        if (U <= maxU) {
-            r.slab = true;
-            r.s.T = T;
-            r.s.kg = kg;
-            r.s.nsets = (G + kg - 1) / kg;
-            r.s.CVw = (int)cv;
-            r.s.RS = RS;
-            r.s.llg = share_lanes(T, kg);
-            r.one = one;
-            r.s.nslab = (long long)N * r.s.nsets;
-            r.U = U <= 1 ? 1 : U <= 2 ? 2 : U <= 4 ? 4 : 8;
-            r.threads = T < 256 ? 256 : T;
-            const int subs = r.threads / T, width = (int)cv * (one && !backward ? 1 : V);
-            r.lds = sizeof(float) * subs * ((backward && !one ? 2 : 1) * (size_t)RS * width + 2 * kg);
-            if (!backward) {
-                const long long b = (r.s.nslab + subs - 1) / subs;
-                if (b >= (1LL << 22)) { r.slab = false; } else r.blocks = (int)b;
-            } else {
-                long long wb = ((long long)N + subs - 1) / subs;
-                const long long most = 2048 / r.s.nsets < 1 ? 1 : 2048 / r.s.nsets;
-                if (wb > most) wb = most;
-                r.walkers = (int)wb * subs;
-                if (wb * r.s.nsets >= (1LL << 22)) r.slab = false; else r.blocks = (int)(wb * r.s.nsets);
-                r.words = 2LL * r.walkers * C;
-            }
-            if (r.lds > 64 * 1024) r.slab = false;
-            if (r.slab) return r;
-        }
-    }
+    if (plan_slab(r, V, N, S, C, G, backward)) return r;
     r = GnPlan();
     GnParts& p = r.p;
+    // tiles of 2^lc vectors: the widest, up to a row of 256, that leaves at most an eighth of the lanes idle; 128 bytes (or the row) otherwise
     const long long cvs = ((long long)C + V - 1) / V;
-    p.tiles = (int)((cvs + 255) / 256);
-    p.CVt = (int)((cvs + p.tiles - 1) / p.tiles);
-    p.RS = 256 / p.CVt;
+    int lc = log2_up(cvs < 256 ? cvs : 256);
+    while (lc > 3 && ((((cvs - 1) >> lc) + 1) << lc) * 8 > cvs * 9) --lc;
+    p.lc = lc;
+    p.tiles = (int)(((cvs - 1) >> lc) + 1);
+    p.rows = 256 >> lc;
+    p.slots = lc > 6 ? p.rows : 4;
     // 8 positions a thread, more where a sample would have over 512 parts.  By the sample's own sizes alone: its result is the same, bit for
     // bit, in a batch of any size.
-    long long P = (S + 8LL * p.RS - 1) / (8LL * p.RS);
+    long long P = (S + 8LL * p.rows - 1) / (8LL * p.rows);
     if (P > 512) P = 512;
-    p.rows = (int)((S + P - 1) / P);
-    p.P = (S + p.rows - 1) / p.rows;
+    p.len = (int)((S + P - 1) / P);
+    p.P = (S + p.len - 1) / p.len;
+    p.tg = (int)(((long long)Cg - 1) / (V << lc) + 2);
+    if (p.tg > p.tiles) p.tg = p.tiles;
     if (backward) {
-        p.llg = share_lanes(256, p.CVt * V);
         r.ab = 2LL * N * p.P * C;
         r.coef = r.ab + 2LL * N * C;
         r.words = r.coef + 2LL * N * G;
     } else {
-        const long long per = ((long long)p.CVt * V + Cg - 1) / Cg + 1;
+        const long long per = ((long long)V << lc) / Cg + 2;
         p.llg = share_lanes(256, (int)(per < G ? per : G));
-        r.words = 3LL * N * p.P * p.tiles * G;
+        r.words = 4LL * N * G * p.P * p.tg;
     }
     return r;
 }
@@ -746,8 +818,7 @@ template <class E, int ACT, bool ONE>
 static int run_slab_bwd(const GnArgs& a, const GnPlan& r, float2* ab, hipStream_t st) {
     const dim3 grid(r.blocks), block(r.threads);
     if (r.U == 1) hipLaunchKernelGGL((gn_slab_bwd_kernel<E, ACT, 1, ONE>), grid, block, r.lds, st, a, r.s, r.walkers, ab);
-    else if (r.U == 2 || !ONE) hipLaunchKernelGGL((gn_slab_bwd_kernel<E, ACT, 2, ONE>), grid, block, r.lds, st, a, r.s, r.walkers, ab);
-    else if constexpr (ONE) hipLaunchKernelGGL((gn_slab_bwd_kernel<E, ACT, 4, true>), grid, block, r.lds, st, a, r.s, r.walkers, ab);
+    else hipLaunchKernelGGL((gn_slab_bwd_kernel<E, ACT, 2, ONE>), grid, block, r.lds, st, a, r.s, r.walkers, ab);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
@@ -755,9 +826,9 @@ template <class E, int ACT>
 static int run_fwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) {
     if (r.slab) return r.one ? run_slab_fwd<E, ACT, true>(a, r, st) : run_slab_fwd<E, ACT, false>(a, r, st);
     const int blocks = a.N * r.p.P * r.p.tiles;
-    hipLaunchKernelGGL(gn_stats_kernel<E>, dim3(blocks), dim3(256), 0, st, a, r.p, ws);
+    hipLaunchKernelGGL(gn_stats_kernel<E>, dim3(blocks), dim3(256), 0, st, a, r.p, (float4*)ws);
     AG2V_CHECK_LAUNCH();
-    hipLaunchKernelGGL(gn_stats_join_kernel, dim3(ceil_div((long long)a.N * a.G, 4)), dim3(256), 0, st, a, r.p.P * r.p.tiles, ws);
+    hipLaunchKernelGGL(gn_stats_join_kernel<E::V>, dim3(ceil_div((long long)a.N * a.G, 4)), dim3(256), 0, st, a, r.p, (const float4*)ws);
     AG2V_CHECK_LAUNCH();
     hipLaunchKernelGGL((gn_apply_kernel<E, ACT>), dim3(blocks), dim3(256), 0, st, a, r.p);
     AG2V_CHECK_LAUNCH();
@@ -778,9 +849,7 @@ static int run_bwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) 
         const int blocks = a.N * r.p.P * r.p.tiles;
         hipLaunchKernelGGL((gn_bwd_sums_kernel<E, ACT>), dim3(blocks), dim3(256), 0, st, a, r.p, part);
         AG2V_CHECK_LAUNCH();
-        int lcw = 0;
-        while (lcw < 8 && (1 << lcw) < a.Cg) ++lcw;
-        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.N * a.G), dim3(256), 0, st, a, r.p.P, lcw, part, sums, coef);
+        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.N * a.G), dim3(256), 0, st, a, r.p.P, log2_up(a.Cg < 256 ? a.Cg : 256), part, sums, coef);
         AG2V_CHECK_LAUNCH();
         if (a.y) hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT>), dim3(blocks), dim3(256), 0, st, a, r.p, coef);
         AG2V_CHECK_LAUNCH();
@@ -800,7 +869,7 @@ static int run_elem(const GnArgs& a, const GnPlan& r, int act, bool backward, fl
 }
 static int run_any(const GnArgs& a, int dtype, int act, bool backward, float* ws, size_t ws_floats, hipStream_t st) {
     const GnPlan r = plan_of(dtype, a.N, a.S, a.C, a.G, backward);
-    if ((r.words && !ws) || ws_floats < (size_t)r.words || ((uintptr_t)ws & 7)) return AG2V_EINVAL;
+    if ((r.words && !ws) || ws_floats < (size_t)r.words || ((uintptr_t)ws & 15)) return AG2V_EINVAL;
     if (!r.slab && (long long)a.N * r.p.P * r.p.tiles >= (1LL << 24)) return AG2V_EINVAL;
     if (dtype == AG2V_F32) return run_elem<ElemF32>(a, r, act, backward, ws, st);
     return dtype == AG2V_BF16 ? run_elem<ElemBF16>(a, r, act, backward, ws, st) : run_elem<ElemF16>(a, r, act, backward, ws, st);
