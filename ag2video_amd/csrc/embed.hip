@@ -8,8 +8,8 @@
 //
 // The gradient, by sizes:
 //   few rows, few tokens    one launch: a workgroup per row of the table picks its tokens out of all n (embed_pick_kernel);
-//   up to RANK_MAX tokens   a token's place in the sorted order is the number of tokens before it: n^2 / 64 compares on the ballot path,
-//                           spread over the whole chip in ONE launch that also clears the table's gradient (embed_rank_kernel);
+//   up to RANK_MAX tokens   a token's place in the sorted order is the number of tokens before it: n^2 compares, spread over the whole
+//                           chip in ONE launch that also clears the table's gradient (embed_rank_kernel);
 //   more                    a stable radix sort, 9 bits a pass, two launches a pass (embed_hist_kernel, embed_scatter_kernel).
 // After a sort, embed_sum_kernel walks equal shares of the sorted order -- a long run of one token costs no more than many short ones --
 // and writes every row whose tokens lie inside one workgroup's share; embed_join_kernel adds the rest up, in order.  No atomics on
@@ -134,55 +134,60 @@ __device__ __forceinline__ void clear_share(char* p, long long bytes, int blk, i
 }
 
 // ---------------------------------------------------------------- gradient: the order by counting
-// Workgroup b ranks tokens [b * RANK_T, ...): rank_i = #{j : k_j < k_i} + #{j < i : k_j = k_i}.  A lane holds k_j, k_i is uniform: a
-// compare and a scalar bit count per 64 pairs.  Tiles of j wholly before i count k_j <= k_i, tiles wholly behind k_j < k_i.
-// Workgroups beyond the ranking ones clear the table's gradient.
-#define RANK_MAX 8192
+// Workgroup b ranks tokens [i0, i0 + 32), i0 = 32 b: rank_i = #{j : k_j < k_i} + #{j < i : k_j = k_i}.  All keys go to LDS; a lane holds k_i
+// (lanes t and t + 32 the same one) and walks its share of j, four broadcast keys a read, a compare and an add with carry each: 2 n^2 / 64
+// vector instructions over the whole chip.  Before i0 equal keys count (k_j < k_i + 1), behind the 32 they do not; the 32 themselves are
+// compared with their positions.  Workgroups beyond the ranking ones clear the table's gradient.
+#define RANK_MAX 16384
 #define RANK_T 32
-__global__ __launch_bounds__(256) void embed_rank_kernel(const void* __restrict__ idx, int wide, long long istride, int* __restrict__ skey,
-                                                         int* __restrict__ order, int n, int V, int pad, int rank_blocks, char* clear,
-                                                         long long clear_bytes) {
+#define RANK_THREADS 1024
+__global__ __launch_bounds__(RANK_THREADS) void embed_rank_kernel(const void* __restrict__ idx, int wide, long long istride, int* __restrict__ skey,
+                                                                  int* __restrict__ order, int n, int V, int pad, int rank_blocks, char* clear,
+                                                                  long long clear_bytes) {
     if ((int)blockIdx.x >= rank_blocks) {
         clear_share(clear, clear_bytes, blockIdx.x - rank_blocks, gridDim.x - rank_blocks);
         return;
     }
-    __shared__ int sh[4][RANK_T];
-    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, i0 = blockIdx.x * RANK_T;
-    int ki[RANK_T], cnt[RANK_T];
-#pragma unroll
-    for (int t = 0; t < RANK_T; ++t) {
-        ki[t] = __builtin_amdgcn_readfirstlane(i0 + t < n ? key_at(idx, wide, istride, i0 + t, V, pad) : 0);
-        cnt[t] = 0;
-    }
-    for (int j0 = wave * 64; j0 < n; j0 += 256) {
-        const int j = j0 + wl;
-        const int kj = j < n ? key_at(idx, wide, istride, j, V, pad) : 0x7fffffff;
-        if (j0 + 64 <= i0) {                   // wholly before: equal ones count
-#pragma unroll
-            for (int t = 0; t < RANK_T; ++t) cnt[t] += __popcll(__ballot(kj <= ki[t]));
-        } else if (j0 >= i0 + RANK_T) {        // wholly behind
-#pragma unroll
-            for (int t = 0; t < RANK_T; ++t) cnt[t] += __popcll(__ballot(kj < ki[t]));
-        } else {
-#pragma unroll
-            for (int t = 0; t < RANK_T; ++t) cnt[t] += __popcll(__ballot(kj < ki[t] || (kj == ki[t] && j < i0 + t)));
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < RANK_T; ++t)
-        if (wl == t) sh[wave][t] = cnt[t];
+    __shared__ __align__(16) int keys[RANK_MAX];
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, i0 = blockIdx.x * RANK_T, t = wl & (RANK_T - 1);
+    const int n4 = (n + 3) & ~3;
+    for (int j = threadIdx.x; j < n4; j += RANK_THREADS) keys[j] = j < n ? key_at(idx, wide, istride, j, V, pad) : 0x7fffffff;
     __syncthreads();
-    const int t = threadIdx.x;
-    if (t < RANK_T && i0 + t < n) {
-        const int r = sh[0][t] + sh[1][t] + sh[2][t] + sh[3][t];
-        skey[r] = key_at(idx, wide, istride, i0 + t, V, pad);
+    const int ki = i0 + t < n ? keys[i0 + t] : 0;
+    // 32 shares of j, in fours: wave w's lanes below 32 take share 2 w, the others share 2 w + 1
+    const int fours = n4 >> 2, share = (fours + 31) >> 5, q0 = (2 * wave + (wl >> 5)) * share, q1 = min(fours, q0 + share);
+    const int qa = i0 >> 2, qb = (i0 + RANK_T) >> 2;
+    int cnt = 0;
+    const auto walk = [&](int from, int to, int limit) {      // keys below `limit` among fours [from, to)
+#pragma unroll 8
+        for (int q = from; q < to; ++q) {
+            const int4 k = *reinterpret_cast<const int4*>(keys + 4 * q);
+            cnt += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+        }
+    };
+    walk(q0, min(q1, qa), ki + 1);
+    walk(max(q0, qb), q1, ki);
+    for (int q = max(q0, qa); q < min(q1, qb); ++q)
+        for (int e = 0; e < 4; ++e) {
+            const int j = 4 * q + e, k = keys[j];
+            cnt += k < ki || (k == ki && j < i0 + t);
+        }
+    cnt += __shfl_xor(cnt, 32, 64);
+    __syncthreads();
+    if (wl < RANK_T) keys[wave * RANK_T + wl] = cnt;
+    __syncthreads();
+    if (threadIdx.x < RANK_T && i0 + t < n) {
+        int r = 0;
+#pragma unroll
+        for (int w = 0; w < RANK_THREADS / 64; ++w) r += keys[w * RANK_T + t];
+        skey[r] = ki;
         order[r] = i0 + t;
     }
 }
 
 // ---------------------------------------------------------------- gradient: the order by radix passes
 // A pass sorts by `bits` <= 9 bits of the key, stably.  Each workgroup owns `rounds` * 2048 consecutive entries.  hist: how often each digit
-// occurs in each workgroup's share, counts[digit][workgroup].  scatter: a workgroup reads all counts, which gives where its entries of
+// occurs in each workgroup's share, counts[workgroup][digit].  scatter: a workgroup reads all counts, which gives where its entries of
 // each digit begin, ranks its entries (within a wave by matching digits over ballots, then over waves, then over rounds) and writes them.
 #define RADIX_BITS 9
 #define RADIX_N (1 << RADIX_BITS)
@@ -210,7 +215,7 @@ __global__ __launch_bounds__(RADIX_THREADS) void embed_hist_kernel(RadixSrc s, i
     const long long lo = (long long)blockIdx.x * rounds * RADIX_TILE, hi = min((long long)n, lo + (long long)rounds * RADIX_TILE);
     for (long long e = lo + threadIdx.x; e < hi; e += RADIX_THREADS) atomicAdd(&h[(radix_key(s, (int)e) >> shift) & mask], 1);   // whole numbers: any order, one result
     __syncthreads();
-    if (threadIdx.x <= mask) counts[threadIdx.x * nb + blockIdx.x] = h[threadIdx.x];
+    counts[blockIdx.x * RADIX_N + threadIdx.x] = h[threadIdx.x];
 }
 
 __global__ __launch_bounds__(RADIX_THREADS) void embed_scatter_kernel(RadixSrc s, int n, int shift, int bits, int rounds, int nb,
@@ -218,14 +223,28 @@ __global__ __launch_bounds__(RADIX_THREADS) void embed_scatter_kernel(RadixSrc s
     constexpr int W = RADIX_THREADS / 64, PER = RADIX_TILE / RADIX_THREADS;
     __shared__ int cnt[W][RADIX_N], base[RADIX_N], wsum[W];
     const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, mask = (1 << bits) - 1, d = threadIdx.x;
+    int key[PER], pos[PER], rank[PER];
+    const auto fetch = [&](int r) {
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const long long e = ((long long)blockIdx.x * rounds + r) * RADIX_TILE + wave * (64 * PER) + q * 64 + wl;
+            key[q] = e < n ? radix_key(s, (int)e) : 0;
+            pos[q] = e < n ? (s.pos ? s.pos[e] : (int)e) : 0;
+        }
+    };
+    fetch(0);
     // where this workgroup's entries of digit d begin: all entries of smaller digits, then those of d in earlier workgroups
     int before = 0, total = 0;
-    if (d <= mask)
-        for (int b = 0; b < nb; ++b) {
-            const int c = counts[d * nb + b];
-            total += c;
-            before += b < (int)blockIdx.x ? c : 0;
+    for (int b0 = 0; b0 < nb; b0 += 32) {
+        int c[32];
+#pragma unroll
+        for (int u = 0; u < 32; ++u) c[u] = b0 + u < nb ? counts[(b0 + u) * RADIX_N + d] : 0;
+#pragma unroll
+        for (int u = 0; u < 32; ++u) {
+            total += c[u];
+            before += b0 + u < (int)blockIdx.x ? c[u] : 0;
         }
+    }
     int scan = total;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -241,14 +260,7 @@ __global__ __launch_bounds__(RADIX_THREADS) void embed_scatter_kernel(RadixSrc s
         for (int w = 0; w < W; ++w) cnt[w][d] = 0;
         __syncthreads();
         const long long e0 = ((long long)blockIdx.x * rounds + r) * RADIX_TILE + wave * (64 * PER);
-        int key[PER], pos[PER], rank[PER];
-#pragma unroll
-        for (int q = 0; q < PER; ++q) {
-            const long long e = e0 + q * 64 + wl;
-            const bool in = e < n;
-            key[q] = in ? radix_key(s, (int)e) : 0;
-            pos[q] = in ? (s.pos ? s.pos[e] : (int)e) : 0;
-        }
+        if (r) fetch(r);
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             const bool in = e0 + q * 64 + wl < n;
@@ -415,6 +427,22 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
     if (open) spill(outside ? part : part + half);
 }
 
+// V of the D floats at p
+template <int V>
+__device__ __forceinline__ void load_part(const float* p, int D, float (&v)[V]) {
+    if (D >= V) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            const u32x4 r = *reinterpret_cast<const u32x4_a4*>(p + k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[k + j] = __uint_as_float(r[j]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = k < D ? p[k] : 0.f;
+    }
+}
+
 // The segments that cross workgroups of embed_sum_kernel: the workgroup where one begins adds its tail and the heads behind it.
 template <class E>
 __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
@@ -437,16 +465,16 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
     const float* heads = a.part + (long long)(blk + 1) * a.D + c;
     float acc[E::V] = {};
     if (c0 < a.D) {
-        for (int q = q0; q < q1; q += 4) {
-            float x[4][E::V];
+        for (int q = q0; q < q1; q += 8) {
+            float x[8][E::V];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 8; ++u) load_part<E::V>(heads + (long long)min(q + u, q1 - 1) * a.D, a.D, x[u]);
 #pragma unroll
-                for (int k = 0; k < E::V; ++k) x[u][k] = q + u < q1 && k < a.D ? heads[(long long)(q + u) * a.D + k] : 0.f;
+            for (int u = 0; u < 8; ++u)
+                if (q + u < q1) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int k = 0; k < E::V; ++k) acc[k] += x[u][k];
+                    for (int k = 0; k < E::V; ++k) acc[k] += x[u][k];
+                }
         }
     }
 #pragma unroll
@@ -455,8 +483,9 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
     if (grp == 0 && c0 < a.D) {
         const float* tail = a.part + (long long)a.nblk * a.D + (long long)blk * a.D + c;
         float v[E::V];
+        load_part<E::V>(tail, a.D, v);
 #pragma unroll
-        for (int k = 0; k < E::V; ++k) v[k] = (k < a.D ? tail[k] : 0.f) + acc[k];
+        for (int k = 0; k < E::V; ++k) v[k] += acc[k];
         for (int g = 1; g < ng; ++g)
 #pragma unroll
             for (int k = 0; k < E::V; ++k) v[k] += sh[k * 256 + (g << a.lsh) + lane];
@@ -542,7 +571,7 @@ static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istr
     SumArgs a = {skey, order, dout, dtable, (float*)(order + p.npad), dstride, n, V, D, p.lsh, p.L, p.nblk, scale};
     if (p.rank) {
         const int rank_blocks = ceil_div(n, RANK_T);
-        hipLaunchKernelGGL(embed_rank_kernel, dim3(rank_blocks + clearers), dim3(256), 0, st, idx, wide, istride, skey, order, n, V, pad, rank_blocks,
+        hipLaunchKernelGGL(embed_rank_kernel, dim3(rank_blocks + clearers), dim3(RANK_THREADS), 0, st, idx, wide, istride, skey, order, n, V, pad, rank_blocks,
                            (char*)dtable, bytes);
         AG2V_CHECK_LAUNCH();
     } else {
