@@ -85,19 +85,31 @@ struct ElemF16 {
     }
 };
 
+// Accesses of tensors beyond these sizes go past the caches (template argument NT).  Results of more than the L2s hold together would leave
+// them full of lines that the next kernel has to write back before it can read: the statistics behind a 134 MB result of group_norm_act
+// took 41 us after ordinary stores and 31 us after these; smaller results stay where the next operator finds them.  Reads that are the last
+// ones of a tensor of over a quarter of the Infinity Cache leave what is still needed there: lookups of 102 MB behind the gradient's sums of
+// as much took 38 us after ordinary loads and 28 us after these; at 67 MB the two did not differ.
+#define AG2V_NT_STORE_BYTES (32LL << 20)
+#define AG2V_NT_LOAD_BYTES (64LL << 20)
+
 // nv of the E::V elements at p (the last vector of a row whose width is no multiple of V); the rest reads as zero.
-template <class E>
+template <class E, bool NT = false>
 __device__ __forceinline__ u32x4 load_vec(const typename E::T* p, int nv) {
-    if (nv >= E::V) return *reinterpret_cast<const typename E::raw*>(p);
+    if (nv >= E::V) {
+        if (NT) return __builtin_nontemporal_load(reinterpret_cast<const typename E::raw*>(p));
+        return *reinterpret_cast<const typename E::raw*>(p);
+    }
     float v[E::V];
 #pragma unroll
     for (int i = 0; i < E::V; ++i) v[i] = i < nv ? E::widen(p[i]) : 0.f;
     return E::pack(v);
 }
-template <class E>
+template <class E, bool NT = false>
 __device__ __forceinline__ void store_vec(typename E::T* p, int nv, const float (&v)[E::V]) {
     if (nv >= E::V) {
-        *reinterpret_cast<typename E::raw*>(p) = E::pack(v);
+        if (NT) __builtin_nontemporal_store(E::pack(v), reinterpret_cast<typename E::raw*>(p));
+        else *reinterpret_cast<typename E::raw*>(p) = E::pack(v);
         return;
     }
 #pragma unroll

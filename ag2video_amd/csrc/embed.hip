@@ -28,7 +28,7 @@ __device__ __forceinline__ int key_at(const void* idx, int wide, long long strid
 // ---------------------------------------------------------------- lookup
 // 2^lsh lanes a row, 16 bytes a lane, four rows in flight a thread.  The last vector of a row whose width is no multiple of the vector
 // moves back to end with the row (its first elements are then written twice, with the same values), so every access is 16 bytes wide.
-template <class E>
+template <class E, bool NT>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__ idx, int wide, long long istride,
                                                         const typename E::T* __restrict__ table, long long tstride,
                                                         typename E::T* __restrict__ out, long long n, int V, int D, float scale, int lsh) {
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__
                 E::unpack(r[u], v);
 #pragma unroll
                 for (int k = 0; k < E::V; ++k) v[k] = in[u] ? v[k] * scale : __builtin_nanf("");
-                if (i0 + u * ng < n) store_vec<E>(out + (i0 + u * ng) * D + c, D, v);
+                if (i0 + u * ng < n) store_vec<E, NT>(out + (i0 + u * ng) * D + c, D, v);
             }
         }
     }
@@ -125,10 +125,12 @@ __global__ __launch_bounds__(256) void embed_pick_kernel(const void* __restrict_
 
 // ---------------------------------------------------------------- gradient: clearing the table (rows that no token names)
 __device__ __forceinline__ void clear_share(char* p, long long bytes, int blk, int nblk) {
-    const long long vecs = bytes >> 4;
+    const long long vecs = bytes >> 4, from = (long long)blk * blockDim.x + threadIdx.x, step = (long long)nblk * blockDim.x;
     const u32x4 z = {0, 0, 0, 0};
-    for (long long i = (long long)blk * blockDim.x + threadIdx.x; i < vecs; i += (long long)nblk * blockDim.x)
-        reinterpret_cast<u32x4_a2*>(p)[i] = z;
+    if (bytes > AG2V_NT_STORE_BYTES)
+        for (long long i = from; i < vecs; i += step) __builtin_nontemporal_store(z, reinterpret_cast<u32x4_a2*>(p) + i);
+    else
+        for (long long i = from; i < vecs; i += step) reinterpret_cast<u32x4_a2*>(p)[i] = z;
     if (blk == 0)
         for (long long i = (vecs << 4) + threadIdx.x * 2; i < bytes; i += blockDim.x * 2) *reinterpret_cast<unsigned short*>(p + i) = 0;
 }
@@ -313,7 +315,7 @@ struct SumArgs {
     int n, V, D, lsh, L, nblk;
     float scale;
 };
-template <class E>
+template <class E, bool NT>
 __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
     constexpr int U = 8;
     __shared__ float head[256 * E::V], tail[256 * E::V];
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
             u32x4 r[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (e + u < e1 && key[u] != a.V && mine) r[u] = load_vec<E>(dout + pos[u] * a.dstride, a.D);
+                if (e + u < e1 && key[u] != a.V && mine) r[u] = load_vec<E, NT>(dout + pos[u] * a.dstride, a.D);
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (e + u < e1) {
@@ -549,8 +551,13 @@ static int run_fwd(const void* idx, int idx_bytes, long long istride, const void
     const long long cv = ((long long)D + E::V - 1) / E::V;
     const int lsh = log2_up(cv < 64 ? cv : 64), rows = (256 >> lsh) * 4;
     const long long blocks = (n + rows - 1) / rows;
-    hipLaunchKernelGGL(embed_fwd_kernel<E>, dim3((int)(blocks < (1 << 20) ? blocks : (1 << 20))), dim3(256), 0, st, idx, idx_bytes == 8, istride,
-                       (const typename E::T*)table, tstride, (typename E::T*)out, n, V, D, scale, lsh);
+    const dim3 grid((int)(blocks < (1 << 20) ? blocks : (1 << 20)));
+    if (n * D * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES)
+        hipLaunchKernelGGL((embed_fwd_kernel<E, true>), grid, dim3(256), 0, st, idx, idx_bytes == 8, istride, (const typename E::T*)table, tstride,
+                           (typename E::T*)out, n, V, D, scale, lsh);
+    else
+        hipLaunchKernelGGL((embed_fwd_kernel<E, false>), grid, dim3(256), 0, st, idx, idx_bytes == 8, istride, (const typename E::T*)table, tstride,
+                           (typename E::T*)out, n, V, D, scale, lsh);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
@@ -590,7 +597,10 @@ static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istr
             s.pos = op;
         }
     }
-    hipLaunchKernelGGL(embed_sum_kernel<E>, dim3(p.nblk * p.slices), dim3(256), 0, st, a);
+    if ((long long)n * D * (long long)sizeof(typename E::T) > AG2V_NT_LOAD_BYTES)
+        hipLaunchKernelGGL((embed_sum_kernel<E, true>), dim3(p.nblk * p.slices), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((embed_sum_kernel<E, false>), dim3(p.nblk * p.slices), dim3(256), 0, st, a);
     AG2V_CHECK_LAUNCH();
     if (p.nblk > 1) {
         hipLaunchKernelGGL(embed_join_kernel<E>, dim3(p.nblk * p.slices), dim3(256), 0, st, a);

@@ -111,6 +111,13 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
         raw[u] = u32x4{0, 0, 0, 0};
         if (on && r < a.S) raw[u] = load_vec<E>(x + r * a.xr, nv);
     }
+    float w[V], b[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = c0 + col * V + k;
+        w[k] = a.w && on && k < nv ? load_any(a.w, a.ptype, c) : 1.f;
+        b[k] = a.b && on && k < nv ? load_any(a.b, a.ptype, c) : 0.f;
+    }
     // per-thread sums to rows[slot][...]
     const auto hand_over = [&](const float (&acc)[V]) {
         float s[NG];
@@ -177,15 +184,11 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
             a.rstd[n * a.G + g0 + g] = 1.f / sqrtf(stat[p.kg + g] * inv + a.eps);
         }
     if (!on) return;
-    float w[V], b[V], rstd[NG];
+    float rstd[NG];
 #pragma unroll
     for (int k = 0; k < NG; ++k) rstd[k] = 1.f / sqrtf(stat[p.kg + gi[k]] * inv + a.eps);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = c0 + col * V + k;
-        w[k] = (a.w && k < nv ? load_any(a.w, a.ptype, c) : 1.f) * rstd[k % NG];
-        b[k] = a.b && k < nv ? load_any(a.b, a.ptype, c) : 0.f;
-    }
+    for (int k = 0; k < V; ++k) w[k] *= rstd[k % NG];
     typename E::T* y = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + col * V;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -456,42 +459,30 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, floa
     }
 }
 
-// A wave per (sample, group): its parts joined pairwise, in fp64.
+// A wave per (sample, group): the mean of its parts' means, then the squares about it, in fp64.
 template <int V>
 __global__ __launch_bounds__(256) void gn_stats_join_kernel(GnArgs a, GnParts p, const float4* part) {
     const int id = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
     if (id >= a.N * a.G) return;
     const int g = id % a.G, tw = V << p.lc, tg = ((g + 1) * a.Cg - 1) / tw - g * a.Cg / tw + 1;    // tiles the group touches
-    double cnt = 0.0, mean = 0.0, m2 = 0.0;
-    const auto join = [&](double cb, double mb, double qb) {
-        if (cb == 0.0) return;
-        const double c = cnt + cb, d = mb - mean, f = cb / c;
-        mean += d * f;
-        m2 += qb + d * d * (cnt * f);
-        cnt = c;
-    };
     const float4* mine = part + (long long)id * p.P * p.tg;
+    double total = 0.0, squares = 0.0;
     for (int i = l; i < p.P * p.tg; i += 64)
-        if (i % p.tg < tg) {
-            const float4 o = mine[i];
-            join(o.x, o.y, o.z);
+        if (p.tg == 1 || i % p.tg < tg) total += (double)mine[i].x * mine[i].y;
+    const double count = (double)a.S * a.Cg, mean = wave_sum_d(total) / count;
+    for (int i = l; i < p.P * p.tg; i += 64)
+        if (p.tg == 1 || i % p.tg < tg) {
+            const double d = mine[i].y - mean;
+            squares += mine[i].z + d * d * mine[i].x;
         }
-    for (int o = 32; o > 0; o >>= 1) {
-        double cb = __shfl_xor(cnt, o, 64), mb = __shfl_xor(mean, o, 64), qb = __shfl_xor(m2, o, 64);
-        if (l & o) {          // both partners form the same pair in the same order
-            const double c = cnt, m = mean, q = m2;
-            cnt = cb; mean = mb; m2 = qb;
-            cb = c; mb = m; qb = q;
-        }
-        join(cb, mb, qb);
-    }
+    squares = wave_sum_d(squares);
     if (l == 0) {
         a.mean[id] = (float)mean;
-        a.rstd[id] = (float)(1.0 / sqrt(m2 / cnt + (double)a.eps));
+        a.rstd[id] = (float)(1.0 / sqrt(squares / count + (double)a.eps));
     }
 }
 
-template <class E, int ACT>
+template <class E, int ACT, bool NT>
 __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p) {
     constexpr int V = E::V, U = 4;
     const GnWhere i = where_of<V>(a, p, blockIdx.x);
@@ -518,7 +509,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p) {
                 E::unpack(raw[u], v);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[k] = act_fwd<ACT>(fmaf(v[k] - mean[k], w[k], b[k]), a.slope);
-                store_vec<E>(y + (long long)(r + u * p.rows) * a.C, i.nv, v);
+                store_vec<E, NT>(y + (long long)(r + u * p.rows) * a.C, i.nv, v);
             }
     }
 }
@@ -643,7 +634,7 @@ __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int l
     }
 }
 
-template <class E, int ACT>
+template <class E, int ACT, bool NT>
 __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef) {
     constexpr int V = E::V, U = 4;
     const GnWhere i = where_of<V>(a, p, blockIdx.x);
@@ -667,8 +658,8 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (r + u * p.rows < i.hi) {
-                rx[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
-                rd[u] = load_vec<E>(dy + (long long)(r + u * p.rows) * a.dr, i.nv);
+                rx[u] = load_vec<E, NT>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
+                rd[u] = load_vec<E, NT>(dy + (long long)(r + u * p.rows) * a.dr, i.nv);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -681,7 +672,7 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
                     const float h = fmaf(v[k], rstd[k], off[k]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                     v[k] = rstd[k] * (w[k] * dz - s1[k] - h * s2[k]);
                 }
-                store_vec<E>(dx + (long long)(r + u * p.rows) * a.C, i.nv, v);
+                store_vec<E, NT>(dx + (long long)(r + u * p.rows) * a.C, i.nv, v);
             }
     }
 }
@@ -830,7 +821,10 @@ static int run_fwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) 
     AG2V_CHECK_LAUNCH();
     hipLaunchKernelGGL(gn_stats_join_kernel<E::V>, dim3(ceil_div((long long)a.N * a.G, 4)), dim3(256), 0, st, a, r.p, (const float4*)ws);
     AG2V_CHECK_LAUNCH();
-    hipLaunchKernelGGL((gn_apply_kernel<E, ACT>), dim3(blocks), dim3(256), 0, st, a, r.p);
+    if ((long long)a.N * a.S * a.C * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES)
+        hipLaunchKernelGGL((gn_apply_kernel<E, ACT, true>), dim3(blocks), dim3(256), 0, st, a, r.p);
+    else
+        hipLaunchKernelGGL((gn_apply_kernel<E, ACT, false>), dim3(blocks), dim3(256), 0, st, a, r.p);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
@@ -851,7 +845,10 @@ static int run_bwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) 
         AG2V_CHECK_LAUNCH();
         hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.N * a.G), dim3(256), 0, st, a, r.p.P, log2_up(a.Cg < 256 ? a.Cg : 256), part, sums, coef);
         AG2V_CHECK_LAUNCH();
-        if (a.y) hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT>), dim3(blocks), dim3(256), 0, st, a, r.p, coef);
+        if (a.y && (long long)a.N * a.S * a.C * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES)      // x and dy together: the bound of loads
+            hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, true>), dim3(blocks), dim3(256), 0, st, a, r.p, coef);
+        else if (a.y)
+            hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, false>), dim3(blocks), dim3(256), 0, st, a, r.p, coef);
         AG2V_CHECK_LAUNCH();
         ab = sums;
     }
