@@ -466,15 +466,32 @@ __global__ __launch_bounds__(256) void gn_stats_join_kernel(GnArgs a, GnParts p,
     if (id >= a.N * a.G) return;
     const int g = id % a.G, tw = V << p.lc, tg = ((g + 1) * a.Cg - 1) / tw - g * a.Cg / tw + 1;    // tiles the group touches
     const float4* mine = part + (long long)id * p.P * p.tg;
+    const int all = p.P * p.tg;
     double total = 0.0, squares = 0.0;
-    for (int i = l; i < p.P * p.tg; i += 64)
-        if (p.tg == 1 || i % p.tg < tg) total += (double)mine[i].x * mine[i].y;
-    const double count = (double)a.S * a.Cg, mean = wave_sum_d(total) / count;
-    for (int i = l; i < p.P * p.tg; i += 64)
-        if (p.tg == 1 || i % p.tg < tg) {
-            const double d = mine[i].y - mean;
-            squares += mine[i].z + d * d * mine[i].x;
+    // eight parts a lane in flight; the first eight stay for the second sum (a map of one tile has at most 512 parts)
+    float4 o[8];
+    const auto fetch = [&](int b) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = b + u * 64 + l;
+            o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < all && (p.tg == 1 || i % p.tg < tg)) o[u] = mine[i];
         }
+    };
+    for (int b = 0; b < all; b += 512) {
+        fetch(b);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) total += (double)o[u].x * o[u].y;
+    }
+    const double count = (double)a.S * a.Cg, mean = wave_sum_d(total) / count;
+    for (int b = 0; b < all; b += 512) {
+        if (all > 512) fetch(b);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const double d = o[u].y - mean;
+            squares += o[u].z + d * d * o[u].x;
+        }
+    }
     squares = wave_sum_d(squares);
     if (l == 0) {
         a.mean[id] = (float)mean;
@@ -634,10 +651,39 @@ __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int l
     }
 }
 
+// dw, db: 32 channels a workgroup, 8 lanes a channel share its `rows` partial sums.
+__device__ __forceinline__ void params_of(const GnArgs& a, int blk, int rows, const float2* ab) {
+    __shared__ float2 sh[256];
+    const int cl = threadIdx.x & 31, slot = threadIdx.x >> 5, c = blk * 32 + cl;
+    float2 v = make_float2(0.f, 0.f);
+    if (c < a.C)
+        for (int r = slot; r < rows; r += 8) {
+            const float2 o = ab[(long long)r * a.C + c];
+            v.x += o.x;
+            v.y += o.y;
+        }
+    sh[threadIdx.x] = v;
+    __syncthreads();
+    if (slot == 0 && c < a.C) {
+        for (int q = 1; q < 8; ++q) {
+            v.x += sh[q * 32 + cl].x;
+            v.y += sh[q * 32 + cl].y;
+        }
+        if (a.dw) store_any(a.dw, a.ptype, c, v.y);
+        if (a.db) store_any(a.db, a.ptype, c, v.x);
+    }
+}
+__global__ __launch_bounds__(256) void gn_params_kernel(GnArgs a, int rows, const float2* ab) { params_of(a, blockIdx.x, rows, ab); }
+
+// dx; the first `pblocks` workgroups sum the parameters' gradients instead.
 template <class E, int ACT, bool NT>
-__global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef) {
+__global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef, int pblocks, const float2* ab) {
     constexpr int V = E::V, U = 4;
-    const GnWhere i = where_of<V>(a, p, blockIdx.x);
+    if ((int)blockIdx.x < pblocks) {
+        params_of(a, blockIdx.x, a.N, ab);
+        return;
+    }
+    const GnWhere i = where_of<V>(a, p, blockIdx.x - pblocks);
     if (i.nv <= 0) return;
     float off[V], rstd[V], w[V], b[V], s1[V], s2[V];
 #pragma unroll
@@ -677,29 +723,6 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
     }
 }
 
-// dw, db: 32 channels a workgroup, 8 lanes a channel share its `rows` partial sums.
-__global__ __launch_bounds__(256) void gn_params_kernel(GnArgs a, int rows, const float2* ab) {
-    __shared__ float2 sh[256];
-    const int cl = threadIdx.x & 31, slot = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-    float2 v = make_float2(0.f, 0.f);
-    if (c < a.C)
-        for (int r = slot; r < rows; r += 8) {
-            const float2 o = ab[(long long)r * a.C + c];
-            v.x += o.x;
-            v.y += o.y;
-        }
-    sh[threadIdx.x] = v;
-    __syncthreads();
-    if (slot == 0 && c < a.C) {
-        for (int q = 1; q < 8; ++q) {
-            v.x += sh[q * 32 + cl].x;
-            v.y += sh[q * 32 + cl].y;
-        }
-        if (a.dw) store_any(a.dw, a.ptype, c, v.y);
-        if (a.db) store_any(a.db, a.ptype, c, v.x);
-    }
-}
-
 // ---------------------------------------------------------------- host
 static int vec_of(int dtype) { return dtype == AG2V_F32 ? ElemF32::V : ElemBF16::V; }
 
@@ -726,7 +749,7 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     const int lc = lcols(kg);
     if (lc > 10 || ((long long)S << lc) > most) return false;
     const bool one = kg == 1 || Cg % V == 0;
-    const int maxT = backward && !one ? 512 : 1024, maxU = backward ? 2 : 8;
+    const int maxT = backward && !one ? 512 : 1024, maxU = backward ? 2 : one ? 8 : 4;
     int T = 64;
     while (T < maxT && (((long long)S << lc) > (long long)T * (maxU < 4 ? maxU : 4) || T < (1 << lc))) T *= 2;
     if (T < (1 << lc)) return false;
@@ -775,9 +798,14 @@ static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
     p.tiles = (int)(((cvs - 1) >> lc) + 1);
     p.rows = 256 >> lc;
     p.slots = lc > 6 ? p.rows : 4;
-    // 8 positions a thread, more where a sample would have over 512 parts.  By the sample's own sizes alone: its result is the same, bit for
-    // bit, in a batch of any size.
-    long long P = (S + 8LL * p.rows - 1) / (8LL * p.rows);
+    // 8 positions a thread; 4 or 2 where a sample would have less than 64 workgroups (3 x 1961 x 90 fp32: the backward pass's sums in 7.0 us
+    // against 12.4); more where it would have over 512 parts.  By the sample's own sizes alone: its result is the
+    // same, bit for bit, in a batch of any size.
+    long long P = 0;
+    for (long long each = 8; each >= 2; each /= 2) {
+        P = (S + each * p.rows - 1) / (each * p.rows);
+        if (P * p.tiles >= 64) break;
+    }
     if (P > 512) P = 512;
     p.len = (int)((S + P - 1) / P);
     p.P = (S + p.len - 1) / p.len;
@@ -800,8 +828,8 @@ static int run_slab_fwd(const GnArgs& a, const GnPlan& r, hipStream_t st) {
     const dim3 grid(r.blocks), block(r.threads);
     if (r.U == 1) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 1, ONE>), grid, block, r.lds, st, a, r.s);
     else if (r.U == 2) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 2, ONE>), grid, block, r.lds, st, a, r.s);
-    else if (r.U == 4) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 4, ONE>), grid, block, r.lds, st, a, r.s);
-    else hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 8, ONE>), grid, block, r.lds, st, a, r.s);
+    else if (r.U == 4 || !ONE) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 4, ONE>), grid, block, r.lds, st, a, r.s);
+    else if constexpr (ONE) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 8, true>), grid, block, r.lds, st, a, r.s);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
@@ -845,11 +873,15 @@ static int run_bwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) 
         AG2V_CHECK_LAUNCH();
         hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.N * a.G), dim3(256), 0, st, a, r.p.P, log2_up(a.Cg < 256 ? a.Cg : 256), part, sums, coef);
         AG2V_CHECK_LAUNCH();
-        if (a.y && (long long)a.N * a.S * a.C * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES)      // x and dy together: the bound of loads
-            hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, true>), dim3(blocks), dim3(256), 0, st, a, r.p, coef);
-        else if (a.y)
-            hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, false>), dim3(blocks), dim3(256), 0, st, a, r.p, coef);
-        AG2V_CHECK_LAUNCH();
+        if (a.y) {
+            const int pblocks = params ? ceil_div(a.C, 32) : 0;
+            if ((long long)a.N * a.S * a.C * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES)      // x and dy together: the bound of loads
+                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, true>), dim3(blocks + pblocks), dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+            else
+                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, false>), dim3(blocks + pblocks), dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+            AG2V_CHECK_LAUNCH();
+            return AG2V_OK;
+        }
         ab = sums;
     }
     if (params) {
