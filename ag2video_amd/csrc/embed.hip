@@ -63,46 +63,49 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__
 }
 
 // ---------------------------------------------------------------- gradient: one launch for few rows and few tokens
-#define PICK_MAX 4096
+#define PICK_MAX 2048
+#define PICK_THREADS 1024
 template <class E>
-__global__ __launch_bounds__(256) void embed_pick_kernel(const void* __restrict__ idx, int wide, long long istride,
+__global__ __launch_bounds__(PICK_THREADS) void embed_pick_kernel(const void* __restrict__ idx, int wide, long long istride,
                                                          const typename E::T* __restrict__ dout, long long dstride,
                                                          typename E::T* __restrict__ dtable, int n, int V, int D, float scale, int pad, int lsh) {
-    __shared__ int list[PICK_MAX], cnt[4];
-    __shared__ float part[256 * E::V];
+    constexpr int W = PICK_THREADS / 64, U = 8;
+    __shared__ int list[PICK_MAX], found[W];
+    __shared__ float part[PICK_THREADS * E::V];
     const int v = blockIdx.x % V, slice = blockIdx.x / V;
     const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
-    // each wave lists the tokens of its quarter, in order
-    const int quarter = (n + 3) / 4, lo = wave * quarter, hi = min(n, lo + quarter);
-    int* mine = list + wave * (PICK_MAX / 4);
-    int found = 0;
-    for (int b = lo; b < hi; b += 64) {
-        const int i = b + wl;
-        const bool hit = i < hi && key_at(idx, wide, istride, i, V, pad) == v;
-        const unsigned long long m = __ballot(hit);
-        if (hit) mine[found + __popcll(m & ((1ull << wl) - 1))] = i;
-        found += __popcll(m);
+    // each wave finds the tokens of its share; their places in the list follow from the waves before
+    const int share_n = (n + W - 1) / W, lo = wave * share_n, hi = min(n, lo + share_n);      // at most 128
+    unsigned long long m[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int i = lo + q * 64 + wl;
+        m[q] = __ballot(i < hi && key_at(idx, wide, istride, i, V, pad) == v);
     }
-    if (wl == 0) cnt[wave] = found;
+    if (wl == 0) found[wave] = __popcll(m[0]) + __popcll(m[1]);
     __syncthreads();
-    const int c1 = cnt[0], c2 = c1 + cnt[1], c3 = c2 + cnt[2], total = c3 + cnt[3];
-    const int lane = threadIdx.x & ((1 << lsh) - 1), grp = threadIdx.x >> lsh, ng = 256 >> lsh;
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        before += w < wave ? found[w] : 0;
+        total += found[w];
+    }
+    const unsigned long long below = (1ull << wl) - 1;
+    if ((m[0] >> wl) & 1) list[before + __popcll(m[0] & below)] = lo + wl;
+    if ((m[1] >> wl) & 1) list[before + __popcll(m[0]) + __popcll(m[1] & below)] = lo + 64 + wl;
+    __syncthreads();
+    const int lane = threadIdx.x & ((1 << lsh) - 1), grp = threadIdx.x >> lsh, ng = PICK_THREADS >> lsh;
     const int c0 = (slice << lsh) * E::V + lane * E::V, c = D < E::V ? 0 : min(c0, D - E::V);
     const int share = (total + ng - 1) / ng, e1 = min(total, (grp + 1) * share);
     float acc[E::V] = {};
     if (c0 < D)
-        for (int e = grp * share; e < e1; e += 4) {
-            u32x4 r[4];
+        for (int e = grp * share; e < e1; e += U) {
+            u32x4 r[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int q = e + u;
-                if (q < e1) {
-                    const int i = q < c1 ? list[q] : q < c2 ? list[PICK_MAX / 4 + q - c1] : q < c3 ? list[PICK_MAX / 2 + q - c2] : list[3 * (PICK_MAX / 4) + q - c3];
-                    r[u] = load_vec<E>(dout + (long long)i * dstride + c, D);
-                }
-            }
+            for (int u = 0; u < U; ++u)
+                if (e + u < e1) r[u] = load_vec<E>(dout + list[e + u] * dstride + c, D);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < U; ++u)
                 if (e + u < e1) {
                     float x[E::V];
                     E::unpack(r[u], x);
@@ -111,12 +114,12 @@ __global__ __launch_bounds__(256) void embed_pick_kernel(const void* __restrict_
                 }
         }
 #pragma unroll
-    for (int k = 0; k < E::V; ++k) part[k * 256 + threadIdx.x] = acc[k];
+    for (int k = 0; k < E::V; ++k) part[k * PICK_THREADS + threadIdx.x] = acc[k];
     __syncthreads();
     if (grp == 0 && c0 < D) {
-        for (int g = 1; g < ng; ++g)
+        for (int g = 1; g * share < total; ++g)
 #pragma unroll
-            for (int k = 0; k < E::V; ++k) acc[k] += part[k * 256 + (g << lsh) + lane];
+            for (int k = 0; k < E::V; ++k) acc[k] += part[k * PICK_THREADS + (g << lsh) + lane];
 #pragma unroll
         for (int k = 0; k < E::V; ++k) acc[k] *= scale;
         store_vec<E>(dtable + (long long)v * D + c, D, acc);
@@ -521,7 +524,8 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
     p.lsh = log2_up(cv < 64 ? cv : 64);
     if (p.lsh < 3) p.lsh = 3;       // at most 32 groups a workgroup
     p.slices = (int)((cv + (1 << p.lsh) - 1) >> p.lsh);
-    p.pick = n <= PICK_MAX && V * p.slices <= 2048 && n * V <= (1LL << 20);
+    // one workgroup may get all n tokens: at most 64 rows a group of lanes then
+    p.pick = n <= 64LL * (PICK_THREADS >> p.lsh) && n <= PICK_MAX && V * p.slices <= 1024;
     if (p.pick) return p;
     p.rank = n <= RANK_MAX;
     // entries a group walks: enough groups for 4096 waves, 8 .. 64; more only where the workgroups' parts would pass 16384
@@ -566,7 +570,7 @@ template <class E>
 static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istride, const void* dout, long long dstride, void* dtable, int n, int V,
                    int D, float scale, int pad, float* workspace, hipStream_t st) {
     if (p.pick) {
-        hipLaunchKernelGGL(embed_pick_kernel<E>, dim3(V * p.slices), dim3(256), 0, st, idx, wide, istride, (const typename E::T*)dout, dstride,
+        hipLaunchKernelGGL(embed_pick_kernel<E>, dim3(V * p.slices), dim3(PICK_THREADS), 0, st, idx, wide, istride, (const typename E::T*)dout, dstride,
                            (typename E::T*)dtable, n, V, D, scale, pad, p.lsh);
         AG2V_CHECK_LAUNCH();
         return AG2V_OK;

@@ -100,23 +100,24 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
     const bool live = slab < p.nslab;
     const int n = live ? (int)(slab / p.nsets) : 0, g0 = live ? (int)(slab - (long long)n * p.nsets) * p.kg : 0;
     const int ng = min(p.kg, a.G - g0), c0 = g0 * a.Cg, W = ng * a.Cg;
-    const int rs = t >> p.lc, col = t & (cols - 1), nv = min(V, W - col * V);
-    const bool on = live && nv > 0;
+    const int rs = t >> p.lc, col = t & (cols - 1);
+    const bool on = live && col * V < W;
+    const int at = W < V ? 0 : min(col * V, W - V), dup = col * V - at;      // (see GnWhere)
     const float inv = 1.f / ((float)a.S * (float)a.Cg);
-    const typename E::T* x = (const typename E::T*)a.x + n * a.xs + c0 + col * V;
+    const typename E::T* x = (const typename E::T*)a.x + n * a.xs + c0 + at;
     u32x4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int r = rs + u * p.rows;
         raw[u] = u32x4{0, 0, 0, 0};
-        if (on && r < a.S) raw[u] = load_vec<E>(x + r * a.xr, nv);
+        if (on && r < a.S) raw[u] = load_vec<E>(x + r * a.xr, W);
     }
     float w[V], b[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int c = c0 + col * V + k;
-        w[k] = a.w && on && k < nv ? load_any(a.w, a.ptype, c) : 1.f;
-        b[k] = a.b && on && k < nv ? load_any(a.b, a.ptype, c) : 0.f;
+        const int c = c0 + at + k;
+        w[k] = a.w && on && at + k < W ? load_any(a.w, a.ptype, c) : 1.f;
+        b[k] = a.b && on && at + k < W ? load_any(a.b, a.ptype, c) : 0.f;
     }
     // per-thread sums to rows[slot][...]
     const auto hand_over = [&](const float (&acc)[V]) {
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
         if (ONE) {
             s[0] = 0.f;
 #pragma unroll
-            for (int k = 0; k < V; ++k) s[0] += acc[k];
+            for (int k = 0; k < V; ++k) s[0] += k >= dup && at + k < W ? acc[k] : 0.f;
         } else {
 #pragma unroll
             for (int k = 0; k < NG; ++k) s[k] = acc[k];
@@ -133,7 +134,8 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
         if (cols > 64 || (t & 63) < cols) {
             const int slot = cols > 64 ? rs : t >> 6;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) rows[slot * width + col * NG + k] = s[k];
+            for (int k = 0; k < NG; ++k)
+                if (ONE || k >= dup) rows[slot * width + (ONE ? col : at + k)] = s[k];
         }
     };
     float acc[V] = {};
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
     int gi[NG];
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-        gi[k] = min(ONE ? col / p.wg : (col * V + k) / a.Cg, ng - 1);
+        gi[k] = min(ONE ? col / p.wg : (at + k) / a.Cg, ng - 1);
         mean[k] = on ? stat[gi[k]] * inv : 0.f;
     }
 #pragma unroll
@@ -170,10 +172,6 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
                 }
             }
     }
-    if (nv < V) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] = k < nv ? acc[k] : 0.f;
-    }
     hand_over(acc);
     __syncthreads();
     if (live) share_sums(rows, p.slots, width, p.wg, ng, p.llg, t, p.T, stat + p.kg);
@@ -189,7 +187,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
     for (int k = 0; k < NG; ++k) rstd[k] = 1.f / sqrtf(stat[p.kg + gi[k]] * inv + a.eps);
 #pragma unroll
     for (int k = 0; k < V; ++k) w[k] *= rstd[k % NG];
-    typename E::T* y = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + col * V;
+    typename E::T* y = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + at;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int r = rs + u * p.rows;
@@ -198,7 +196,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
             E::unpack(raw[u], v);
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] = act_fwd<ACT>(fmaf(v[k] - mean[k % NG], w[k], b[k]), a.slope);
-            store_vec<E>(y + (long long)r * a.C, nv, v);
+            store_vec<E>(y + (long long)r * a.C, W, v);
         }
     }
 }
@@ -219,37 +217,38 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
     float* stat = r1 + area;
     const int blk = xcd_remap(blockIdx.x, gridDim.x), set = blk % p.nsets, walker = blk / p.nsets * subs + sub;
     const int g0 = set * p.kg, ng = min(p.kg, a.G - g0), c0 = g0 * a.Cg, W = ng * a.Cg;
-    const int rs = t >> p.lc, col = t & (cols - 1), nv = min(V, W - col * V);
-    const bool on = nv > 0, writes = cols > 64 || (t & 63) < cols;
+    const int rs = t >> p.lc, col = t & (cols - 1);
+    const bool on = col * V < W, writes = cols > 64 || (t & 63) < cols;
+    const int at = W < V ? 0 : min(col * V, W - V), dup = col * V - at;      // (see GnWhere)
     const int slot = cols > 64 ? rs : t >> 6;
     const float inv = 1.f / ((float)a.S * (float)a.Cg);
     float w[V], b[V], A[V], B[V];
     int gi[NG];
 #pragma unroll
-    for (int k = 0; k < NG; ++k) gi[k] = min(ONE ? col / p.wg : (col * V + k) / a.Cg, ng - 1);
+    for (int k = 0; k < NG; ++k) gi[k] = min(ONE ? col / p.wg : (at + k) / a.Cg, ng - 1);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int c = c0 + col * V + k;
-        w[k] = a.w && k < nv ? load_any(a.w, a.ptype, c) : 1.f;
-        b[k] = a.b && k < nv ? load_any(a.b, a.ptype, c) : 0.f;
+        const int c = c0 + at + k;
+        w[k] = a.w && on && at + k < W ? load_any(a.w, a.ptype, c) : 1.f;
+        b[k] = a.b && on && at + k < W ? load_any(a.b, a.ptype, c) : 0.f;
         A[k] = B[k] = 0.f;
     }
     for (int n0 = blk / p.nsets * subs; n0 < a.N; n0 += walkers) {
         const int n = n0 + sub;
         const bool live = n < a.N, here = on && live;
         u32x4 rx[U], rd[U];
-        const typename E::T* x = (const typename E::T*)a.x + (long long)n * a.xs + c0 + col * V;
-        const typename E::T* dy = (const typename E::T*)a.dy + (long long)n * a.ds + c0 + col * V;
+        const typename E::T* x = (const typename E::T*)a.x + (long long)n * a.xs + c0 + at;
+        const typename E::T* dy = (const typename E::T*)a.dy + (long long)n * a.ds + c0 + at;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int r = rs + u * p.rows;
             rx[u] = rd[u] = u32x4{0, 0, 0, 0};
             if (here && r < a.S) {
-                rx[u] = load_vec<E>(x + r * a.xr, nv);
-                rd[u] = load_vec<E>(dy + r * a.dr, nv);
+                rx[u] = load_vec<E>(x + r * a.xr, W);
+                rd[u] = load_vec<E>(dy + r * a.dr, W);
             }
         }
-        float off[NG], rstd[NG], g1[NG] = {}, g2[NG] = {};      // h = x rstd + off; g1, g2: sums of w dz and w dz h
+        float off[NG], rstd[NG], sA[V] = {}, sB[V] = {}, g1[NG] = {}, g2[NG] = {};      // h = x rstd + off; sums of dz, dz h; of w dz, w dz h
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
             rstd[k] = here ? a.rstd[(long long)n * a.G + g0 + gi[k]] : 0.f;
@@ -264,23 +263,31 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = fmaf(v[k], rstd[k % NG], off[k % NG]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope), e = w[k] * dz;
-                        A[k] += dz;
-                        B[k] = fmaf(dz, h, B[k]);
-                        g1[k % NG] += e;
-                        g2[k % NG] = fmaf(e, h, g2[k % NG]);
+                        const float h = fmaf(v[k], rstd[k % NG], off[k % NG]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                        sA[k] += dz;
+                        sB[k] = fmaf(dz, h, sB[k]);
                     }
                 }
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                A[k] += sA[k];
+                B[k] += sB[k];
+                if (k >= dup) {
+                    g1[k % NG] = fmaf(w[k], sA[k], g1[k % NG]);
+                    g2[k % NG] = fmaf(w[k], sB[k], g2[k % NG]);
+                }
+            }
         }
         if (a.y) {
             same_vector_sums(g1, cols);
             same_vector_sums(g2, cols);
             if (writes) {
 #pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    r1[slot * gwidth + col * NG + k] = g1[k];
-                    r2[slot * gwidth + col * NG + k] = g2[k];
-                }
+                for (int k = 0; k < NG; ++k)
+                    if (ONE || k >= dup) {
+                        r1[slot * gwidth + (ONE ? col : at + k)] = g1[k];
+                        r2[slot * gwidth + (ONE ? col : at + k)] = g2[k];
+                    }
             }
             __syncthreads();
             if (live) {
@@ -290,7 +297,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
             __syncthreads();
         }
         if (here && a.y) {
-            typename E::T* dx = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + col * V;
+            typename E::T* dx = (typename E::T*)a.y + (long long)n * a.S * a.C + c0 + at;
             // (the values above are computed again: kept, they would not fit the registers)
 #pragma unroll
             for (int u = 0; u < U; ++u) asm volatile("" : "+v"(rx[u]), "+v"(rd[u]));
@@ -311,7 +318,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
                         const float h = fmaf(v[k], rstd[k % NG], off[k % NG]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                         v[k] = rstd[k % NG] * (w[k] * dz - g1[k % NG] - h * g2[k % NG]);
                     }
-                    store_vec<E>(dx + (long long)r * a.C, nv, v);
+                    store_vec<E>(dx + (long long)r * a.C, W, v);
                 }
             }
         }
@@ -324,7 +331,8 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
         __syncthreads();
         if (writes) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) r1[slot * width + col * V + k] = half ? B[k] : A[k];
+            for (int k = 0; k < V; ++k)
+                if (k >= dup) r1[slot * width + at + k] = half ? B[k] : A[k];
         }
         __syncthreads();
         for (int c = t; c < W; c += p.T) {
@@ -340,8 +348,11 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
 struct GnParts {
     int tiles, lc, rows, slots, len, P, tg, llg;    // P: parts a sample; tg: tiles a group may touch
 };
+// The last vector of a row whose width is no multiple of the vector moves back to end with the row: every access is 16 bytes wide, the
+// `dup` elements it shares with the vector before are written twice with the same values and left out of the sums.
 struct GnWhere {
-    int tile, n, q, rs, col, c0, W, nv, lo, hi;
+    int tile, n, q, rs, c0, W, c, dup, lo, hi;      // c: first channel of the thread's vector
+    bool on;
 };
 template <int V>
 __device__ __forceinline__ GnWhere where_of(const GnArgs& a, const GnParts& p, int blk) {
@@ -351,10 +362,12 @@ __device__ __forceinline__ GnWhere where_of(const GnArgs& a, const GnParts& p, i
     i.n = np / p.P;
     i.q = np - i.n * p.P;
     i.rs = threadIdx.x >> p.lc;
-    i.col = threadIdx.x & ((1 << p.lc) - 1);
     i.c0 = (i.tile * V) << p.lc;
     i.W = min(V << p.lc, a.C - i.c0);
-    i.nv = min(V, i.W - i.col * V);
+    const int c = i.c0 + (threadIdx.x & ((1 << p.lc) - 1)) * V;
+    i.on = c < a.C;
+    i.c = a.C < V ? 0 : min(c, a.C - V);
+    i.dup = c - i.c;
     i.lo = i.q * p.len;
     i.hi = min(a.S, i.lo + p.len);
     return i;
@@ -370,16 +383,15 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, floa
     __shared__ float sm[4 * 64 * V], sq[4 * 64 * V], sn[4];      // [slot][width]
     const GnWhere i = where_of<V>(a, p, blockIdx.x);
     const int cols = 1 << p.lc, width = cols * V;
-    const bool on = i.nv > 0;
-    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c0 + i.col * V;
+    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
     float mean[V] = {}, s[V] = {}, m[V] = {};
     int count = 0;
-    if (on && i.lo + i.rs < i.hi) {
+    if (i.on && i.lo + i.rs < i.hi) {
         for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
             u32x4 raw[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r + u * p.rows < i.hi) raw[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
+                if (r + u * p.rows < i.hi) raw[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, a.C);
             if (count == 0) E::unpack(raw[0], mean);
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -418,11 +430,12 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, floa
     const int slot = cols > 64 ? i.rs : threadIdx.x >> 6;
     if (cols > 64 || (threadIdx.x & 63) < cols) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            sm[slot * width + i.col * V + k] = mean[k];
-            sq[slot * width + i.col * V + k] = m[k];
-        }
-        if (i.col == 0) sn[slot] = nn;
+        for (int k = 0; k < V; ++k)
+            if (i.on && k >= i.dup && i.c + k < a.C) {
+                sm[slot * width + i.c - i.c0 + k] = mean[k];
+                sq[slot * width + i.c - i.c0 + k] = m[k];
+            }
+        if ((threadIdx.x & (cols - 1)) == 0) sn[slot] = nn;
     }
     __syncthreads();
     // the slots of a channel, to slot 0
@@ -503,22 +516,22 @@ template <class E, int ACT, bool NT>
 __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p) {
     constexpr int V = E::V, U = 4;
     const GnWhere i = where_of<V>(a, p, blockIdx.x);
-    if (i.nv <= 0) return;
+    if (!i.on) return;
     float mean[V], w[V], b[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int c = min(i.c0 + i.col * V + k, a.C - 1), g = i.n * a.G + c / a.Cg;
+        const int c = min(i.c + k, a.C - 1), g = i.n * a.G + c / a.Cg;
         mean[k] = a.mean[g];
         w[k] = (a.w ? load_any(a.w, a.ptype, c) : 1.f) * a.rstd[g];
         b[k] = a.b ? load_any(a.b, a.ptype, c) : 0.f;
     }
-    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c0 + i.col * V;
-    typename E::T* y = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c0 + i.col * V;
+    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
+    typename E::T* y = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c;
     for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
         u32x4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (r + u * p.rows < i.hi) raw[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
+            if (r + u * p.rows < i.hi) raw[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, a.C);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (r + u * p.rows < i.hi) {
@@ -526,7 +539,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p) {
                 E::unpack(raw[u], v);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[k] = act_fwd<ACT>(fmaf(v[k] - mean[k], w[k], b[k]), a.slope);
-                store_vec<E, NT>(y + (long long)(r + u * p.rows) * a.C, i.nv, v);
+                store_vec<E, NT>(y + (long long)(r + u * p.rows) * a.C, a.C, v);
             }
     }
 }
@@ -539,25 +552,25 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
     const GnWhere i = where_of<V>(a, p, blockIdx.x);
     const int cols = 1 << p.lc, width = cols * V;
     float A[V] = {}, B[V] = {};
-    if (i.nv > 0) {
+    if (i.on) {
         float off[V], rstd[V], w[V], b[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const int c = min(i.c0 + i.col * V + k, a.C - 1), g = i.n * a.G + c / a.Cg;
+            const int c = min(i.c + k, a.C - 1), g = i.n * a.G + c / a.Cg;
             rstd[k] = a.rstd[g];
             off[k] = -a.mean[g] * rstd[k];
             w[k] = a.w ? load_any(a.w, a.ptype, c) : 1.f;
             b[k] = a.b ? load_any(a.b, a.ptype, c) : 0.f;
         }
-        const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c0 + i.col * V;
-        const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c0 + i.col * V;
+        const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
+        const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c;
         for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
             u32x4 rx[U], rd[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (r + u * p.rows < i.hi) {
-                    rx[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
-                    rd[u] = load_vec<E>(dy + (long long)(r + u * p.rows) * a.dr, i.nv);
+                    rx[u] = load_vec<E>(x + (long long)(r + u * p.rows) * a.xr, a.C);
+                    rd[u] = load_vec<E>(dy + (long long)(r + u * p.rows) * a.dr, a.C);
                 }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -579,10 +592,11 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
     if (cols > 64 || (threadIdx.x & 63) < cols) {
         const int slot = cols > 64 ? i.rs : threadIdx.x >> 6;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            r1[slot * width + i.col * V + k] = A[k];
-            r2[slot * width + i.col * V + k] = B[k];
-        }
+        for (int k = 0; k < V; ++k)
+            if (i.on && k >= i.dup && i.c + k < a.C) {
+                r1[slot * width + i.c - i.c0 + k] = A[k];
+                r2[slot * width + i.c - i.c0 + k] = B[k];
+            }
     }
     __syncthreads();
     for (int c = threadIdx.x; c < i.W; c += 256) {
@@ -684,11 +698,11 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
         return;
     }
     const GnWhere i = where_of<V>(a, p, blockIdx.x - pblocks);
-    if (i.nv <= 0) return;
+    if (!i.on) return;
     float off[V], rstd[V], w[V], b[V], s1[V], s2[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int c = min(i.c0 + i.col * V + k, a.C - 1), g = i.n * a.G + c / a.Cg;
+        const int c = min(i.c + k, a.C - 1), g = i.n * a.G + c / a.Cg;
         rstd[k] = a.rstd[g];
         off[k] = -a.mean[g] * rstd[k];
         w[k] = a.w ? load_any(a.w, a.ptype, c) : 1.f;
@@ -696,16 +710,16 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
         s1[k] = coef[g].x;
         s2[k] = coef[g].y;
     }
-    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c0 + i.col * V;
-    const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c0 + i.col * V;
-    typename E::T* dx = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c0 + i.col * V;
+    const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
+    const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c;
+    typename E::T* dx = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c;
     for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
         u32x4 rx[U], rd[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (r + u * p.rows < i.hi) {
-                rx[u] = load_vec<E, NT>(x + (long long)(r + u * p.rows) * a.xr, i.nv);
-                rd[u] = load_vec<E, NT>(dy + (long long)(r + u * p.rows) * a.dr, i.nv);
+                rx[u] = load_vec<E, NT>(x + (long long)(r + u * p.rows) * a.xr, a.C);
+                rd[u] = load_vec<E, NT>(dy + (long long)(r + u * p.rows) * a.dr, a.C);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -718,7 +732,7 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
                     const float h = fmaf(v[k], rstd[k], off[k]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                     v[k] = rstd[k] * (w[k] * dz - s1[k] - h * s2[k]);
                 }
-                store_vec<E, NT>(dx + (long long)(r + u * p.rows) * a.C, i.nv, v);
+                store_vec<E, NT>(dx + (long long)(r + u * p.rows) * a.C, a.C, v);
             }
     }
 }
