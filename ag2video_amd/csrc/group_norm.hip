@@ -37,6 +37,51 @@ __device__ __forceinline__ float act_bwd(float dy, float z, float slope) {
     return dy;
 }
 
+// V parameters from channel c of C on, `none` where there are none
+template <class E>
+__device__ __forceinline__ void load_params(const void* p, int ptype, int c, int C, float none, float (&v)[E::V]) {
+    constexpr int V = E::V;
+    if (!p) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = none;
+    } else if (c + V > C) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = c + k < C ? load_any(p, ptype, c + k) : none;
+    } else if (ptype == AG2V_F32) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            const u32x4 r = *reinterpret_cast<const u32x4_a4*>((const float*)p + c + k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[k + j] = __uint_as_float(r[j]);
+        }
+    } else {            // the maps' own type
+        E::unpack(load_vec<E>((const typename E::T*)p + c, V), v);
+    }
+}
+// mean and 1 / std of V channels from c on
+template <int V>
+__device__ __forceinline__ void load_stats(const GnArgs& a, int n, int c, float (&mean)[V], float (&rstd)[V], const float2* coef = nullptr, float2* cf = nullptr) {
+    if (a.Cg % V == 0 && c % V == 0) {
+        const int g = n * a.G + c / a.Cg;
+        const float m = a.mean[g], r = a.rstd[g];
+        const float2 f = coef ? coef[g] : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            mean[k] = m;
+            rstd[k] = r;
+            if (coef) cf[k] = f;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int g = n * a.G + min(c + k, a.C - 1) / a.Cg;
+            mean[k] = a.mean[g];
+            rstd[k] = a.rstd[g];
+            if (coef) cf[k] = coef[g];
+        }
+    }
+}
+
 // ---------------------------------------------------------------- layout shared by the kernels
 // Channels are walked as rows of 16-byte vectors.  `cols` vectors side by side -- a power of two, the ones beyond the slab or tile idle --
 // and threads / cols rows at a time: thread t works on vector t % cols of row t / cols, t / cols + rows at a time, ...  Lanes of one wave
@@ -113,12 +158,8 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
         if (on && r < a.S) raw[u] = load_vec<E>(x + r * a.xr, W);
     }
     float w[V], b[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = c0 + at + k;
-        w[k] = a.w && on && at + k < W ? load_any(a.w, a.ptype, c) : 1.f;
-        b[k] = a.b && on && at + k < W ? load_any(a.b, a.ptype, c) : 0.f;
-    }
+    load_params<E>(a.w, a.ptype, c0 + at, a.C, 1.f, w);
+    load_params<E>(a.b, a.ptype, c0 + at, a.C, 0.f, b);
     // per-thread sums to rows[slot][...]
     const auto hand_over = [&](const float (&acc)[V]) {
         float s[NG];
@@ -226,13 +267,10 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
     int gi[NG];
 #pragma unroll
     for (int k = 0; k < NG; ++k) gi[k] = min(ONE ? col / p.wg : (at + k) / a.Cg, ng - 1);
+    load_params<E>(a.w, a.ptype, c0 + at, a.C, 1.f, w);
+    load_params<E>(a.b, a.ptype, c0 + at, a.C, 0.f, b);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = c0 + at + k;
-        w[k] = a.w && on && at + k < W ? load_any(a.w, a.ptype, c) : 1.f;
-        b[k] = a.b && on && at + k < W ? load_any(a.b, a.ptype, c) : 0.f;
-        A[k] = B[k] = 0.f;
-    }
+    for (int k = 0; k < V; ++k) A[k] = B[k] = 0.f;
     for (int n0 = blk / p.nsets * subs; n0 < a.N; n0 += walkers) {
         const int n = n0 + sub;
         const bool live = n < a.N, here = on && live;
@@ -357,6 +395,8 @@ struct GnWhere {
 template <int V>
 __device__ __forceinline__ GnWhere where_of(const GnArgs& a, const GnParts& p, int blk) {
     GnWhere i;
+    // rows of neighbouring tiles share cache lines: tiles of a part, and neighbouring parts, run on one XCD
+    blk = xcd_remap(blk, p.tiles * p.P * a.N);
     i.tile = blk % p.tiles;
     const int np = blk / p.tiles;
     i.n = np / p.P;
@@ -517,14 +557,12 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p) {
     constexpr int V = E::V, U = 4;
     const GnWhere i = where_of<V>(a, p, blockIdx.x);
     if (!i.on) return;
-    float mean[V], w[V], b[V];
+    float mean[V], rstd[V], w[V], b[V];
+    load_params<E>(a.w, a.ptype, i.c, a.C, 1.f, w);
+    load_params<E>(a.b, a.ptype, i.c, a.C, 0.f, b);
+    load_stats<V>(a, i.n, i.c, mean, rstd);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = min(i.c + k, a.C - 1), g = i.n * a.G + c / a.Cg;
-        mean[k] = a.mean[g];
-        w[k] = (a.w ? load_any(a.w, a.ptype, c) : 1.f) * a.rstd[g];
-        b[k] = a.b ? load_any(a.b, a.ptype, c) : 0.f;
-    }
+    for (int k = 0; k < V; ++k) w[k] *= rstd[k];
     const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
     typename E::T* y = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c;
     for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
@@ -554,14 +592,11 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
     float A[V] = {}, B[V] = {};
     if (i.on) {
         float off[V], rstd[V], w[V], b[V];
+        load_params<E>(a.w, a.ptype, i.c, a.C, 1.f, w);
+        load_params<E>(a.b, a.ptype, i.c, a.C, 0.f, b);
+        load_stats<V>(a, i.n, i.c, off, rstd);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const int c = min(i.c + k, a.C - 1), g = i.n * a.G + c / a.Cg;
-            rstd[k] = a.rstd[g];
-            off[k] = -a.mean[g] * rstd[k];
-            w[k] = a.w ? load_any(a.w, a.ptype, c) : 1.f;
-            b[k] = a.b ? load_any(a.b, a.ptype, c) : 0.f;
-        }
+        for (int k = 0; k < V; ++k) off[k] = -off[k] * rstd[k];
         const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
         const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c;
         for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
@@ -699,17 +734,13 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
     }
     const GnWhere i = where_of<V>(a, p, blockIdx.x - pblocks);
     if (!i.on) return;
-    float off[V], rstd[V], w[V], b[V], s1[V], s2[V];
+    float off[V], rstd[V], w[V], b[V];
+    float2 cf[V];
+    load_params<E>(a.w, a.ptype, i.c, a.C, 1.f, w);
+    load_params<E>(a.b, a.ptype, i.c, a.C, 0.f, b);
+    load_stats<V>(a, i.n, i.c, off, rstd, coef, cf);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = min(i.c + k, a.C - 1), g = i.n * a.G + c / a.Cg;
-        rstd[k] = a.rstd[g];
-        off[k] = -a.mean[g] * rstd[k];
-        w[k] = a.w ? load_any(a.w, a.ptype, c) : 1.f;
-        b[k] = a.b ? load_any(a.b, a.ptype, c) : 0.f;
-        s1[k] = coef[g].x;
-        s2[k] = coef[g].y;
-    }
+    for (int k = 0; k < V; ++k) off[k] = -off[k] * rstd[k];
     const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
     const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c;
     typename E::T* dx = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c;
@@ -730,7 +761,7 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const float h = fmaf(v[k], rstd[k], off[k]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
-                    v[k] = rstd[k] * (w[k] * dz - s1[k] - h * s2[k]);
+                    v[k] = rstd[k] * (w[k] * dz - cf[k].x - h * cf[k].y);
                 }
                 store_vec<E, NT>(dx + (long long)(r + u * p.rows) * a.C, a.C, v);
             }
@@ -761,6 +792,9 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     int kg = 1;
     while (kg < G && (long long)kg * Cg < 8 * V && lcols(kg + 1) <= 3 && ((long long)S << lcols(kg + 1)) <= most) ++kg;
     const int lc = lcols(kg);
+    // narrow rows that are no whole vectors: every cache line would be read by many slabs, in pieces (11 x 4181 x 45 fp32 in 15 groups: 49 us a
+    // training pass; rows of one vector, 8 x 4096 x 256 fp16 in 32 groups, are as fast here, 20.8 us forward, as in parts, 23 us)
+    if (kg < G && Cg % V && (long long)kg * Cg < 4 * V) return false;
     if (lc > 10 || ((long long)S << lc) > most) return false;
     const bool one = kg == 1 || Cg % V == 0;
     const int maxT = backward && !one ? 512 : 1024, maxU = backward ? 2 : one ? 8 : 4;
@@ -804,10 +838,10 @@ static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
     if (plan_slab(r, V, N, S, C, G, backward)) return r;
     r = GnPlan();
     GnParts& p = r.p;
-    // tiles of 2^lc vectors: the widest, up to a row of 256, that leaves at most an eighth of the lanes idle; 128 bytes (or the row) otherwise
+    // tiles of 2^lc vectors: the widest, up to a row of 256, that leaves at most an eighth of the lanes idle; 64 bytes (or the row) otherwise
     const long long cvs = ((long long)C + V - 1) / V;
     int lc = log2_up(cvs < 256 ? cvs : 256);
-    while (lc > 3 && ((((cvs - 1) >> lc) + 1) << lc) * 8 > cvs * 9) --lc;
+    while (lc > 2 && ((((cvs - 1) >> lc) + 1) << lc) * 8 > cvs * 9) --lc;
     p.lc = lc;
     p.tiles = (int)(((cvs - 1) >> lc) + 1);
     p.rows = 256 >> lc;
@@ -920,6 +954,7 @@ static int run_any(const GnArgs& a, int dtype, int act, bool backward, float* ws
 
 static bool sizes_ok(int dtype, int ptype, int N, int S, int C, int groups, int act) {
     if (dtype < AG2V_F32 || dtype > AG2V_F16 || ptype < AG2V_F32 || ptype > AG2V_F16 || act < ACT_NONE || act > ACT_LRELU) return false;
+    if (ptype != AG2V_F32 && ptype != dtype) return false;
     if (N <= 0 || S <= 0 || C <= 0 || groups <= 0 || C % groups) return false;
     return (long long)N * groups < (1LL << 24);
 }

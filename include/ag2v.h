@@ -386,7 +386,7 @@ int ag2v_embed_bwd(int dtype, const void* idx, int idx_bytes, long long idx_stri
                    void* stream);
 
 /* Group norm with an activation, channels last: x[N,S,C] (strides x_sample / x_row in elements, channels adjacent), y contiguous,
- * weight / bias [C] of param_dtype or NULL (1 / 0), mean / rstd fp32 [N,groups] written for the backward pass.
+ * weight / bias [C] of param_dtype (AG2V_F32 or dtype) or NULL (1 / 0), mean / rstd fp32 [N,groups] written for the backward pass.
  * act: 0 none, 1 silu, 2 leaky relu of `slope`.  Backward: dx (contiguous), dweight, dbias (param_dtype); each may be NULL.
  * No atomics: equal calls give equal bits.  workspace: ag2v_group_norm_workspace_floats(..., backward) floats. */
 size_t ag2v_group_norm_workspace_floats(int dtype, int N, int S, int C, int groups, int backward);
