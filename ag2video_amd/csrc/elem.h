@@ -117,6 +117,40 @@ __device__ __forceinline__ void store_vec(typename E::T* p, int nv, const float 
         if (i < nv) p[i] = E::narrow(v[i]);
 }
 
+// The last vector of a row whose width is no multiple of V is loaded so that it ends with the row; its first `dup` elements are the vector
+// before's, and only the others are stored (that vector's lane may round its own differently: the compiler is free to fuse a product into the
+// conversion for one element of a vector and not for another).
+template <class E, bool NT = false>
+__device__ __forceinline__ void store_tail(typename E::T* p, int dup, int width, const float (&v)[E::V]) {
+    if (dup == 0 || width < E::V) {
+        store_vec<E, NT>(p, width, v);
+        return;
+    }
+    typedef unsigned u32_a2 __attribute__((aligned(2), may_alias));
+    typedef unsigned long long u64_a2 __attribute__((aligned(2), may_alias));
+    const u32x4 r = E::pack(v);
+    unsigned long long lo = r[0] | (unsigned long long)r[1] << 32, hi = r[2] | (unsigned long long)r[3] << 32;
+    const int bits = dup * (int)sizeof(typename E::T) * 8, bytes = 16 - (bits >> 3);
+    if (bits >= 64) {
+        lo = hi >> (bits - 64);
+    } else {
+        lo = lo >> bits | hi << (64 - bits);
+        hi >>= bits;
+    }
+    char* q = (char*)(p + dup);
+    if (bytes & 8) {
+        *reinterpret_cast<u64_a2*>(q) = lo;
+        lo = hi;
+        q += 8;
+    }
+    if (bytes & 4) {
+        *reinterpret_cast<u32_a2*>(q) = (unsigned)lo;
+        lo >>= 32;
+        q += 4;
+    }
+    if (bytes & 2) *reinterpret_cast<unsigned short*>(q) = (unsigned short)lo;
+}
+
 // One value of a tensor whose type is a kernel argument (the same branch for every lane).
 __device__ __forceinline__ float load_any(const void* p, int dtype, long long i) {
     if (dtype == AG2V_F32) return ((const float*)p)[i];

@@ -25,9 +25,23 @@ __device__ __forceinline__ int key_at(const void* idx, int wide, long long strid
     return v >= 0 && v < V && v != pad ? (int)v : V;
 }
 
+// The last vector of a row whose width is no multiple of V ends with the row: the elements it shares with the vector before are written
+// twice, with the same bits.  They are sums in one order and one product, and the product is rounded to fp32 before the conversion (the
+// compiler would fuse the two for some elements of a vector and not for others).
+template <class E, bool NT = false>
+__device__ __forceinline__ void store_row(typename E::T* p, int width, const float (&x)[E::V]) {
+    float v[E::V];
+#pragma unroll
+    for (int k = 0; k < E::V; ++k) {
+        v[k] = x[k];
+        asm volatile("" : "+v"(v[k]));
+    }
+    store_vec<E, NT>(p, width, v);
+}
+
 // ---------------------------------------------------------------- lookup
 // 2^lsh lanes a row, 16 bytes a lane, four rows in flight a thread.  The last vector of a row whose width is no multiple of the vector
-// moves back to end with the row (its first elements are then written twice, with the same values), so every access is 16 bytes wide.
+// moves back to end with the row (store_row).
 template <class E, bool NT>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__ idx, int wide, long long istride,
                                                         const typename E::T* __restrict__ table, long long tstride,
@@ -56,7 +70,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__
                 E::unpack(r[u], v);
 #pragma unroll
                 for (int k = 0; k < E::V; ++k) v[k] = in[u] ? v[k] * scale : __builtin_nanf("");
-                if (i0 + u * ng < n) store_vec<E, NT>(out + (i0 + u * ng) * D + c, D, v);
+                if (i0 + u * ng < n) store_row<E, NT>(out + (i0 + u * ng) * D + c, D, v);
             }
         }
     }
@@ -122,7 +136,7 @@ __global__ __launch_bounds__(PICK_THREADS) void embed_pick_kernel(const void* __
             for (int k = 0; k < E::V; ++k) acc[k] += part[k * PICK_THREADS + (g << lsh) + lane];
 #pragma unroll
         for (int k = 0; k < E::V; ++k) acc[k] *= scale;
-        store_vec<E>(dtable + (long long)v * D + c, D, acc);
+        store_row<E>(dtable + (long long)v * D + c, D, acc);
     }
 }
 
@@ -345,7 +359,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
                 float v[E::V];
 #pragma unroll
                 for (int k = 0; k < E::V; ++k) v[k] = acc[k] * a.scale;
-                store_vec<E>(dtable + (long long)cur * a.D, a.D, v);
+                store_row<E>(dtable + (long long)cur * a.D, a.D, v);
             }
         };
         for (long long e = e0; e < e1; e += U) {
@@ -417,7 +431,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
                     float v[E::V];
 #pragma unroll
                     for (int k = 0; k < E::V; ++k) v[k] = acc[k] * a.scale;
-                    store_vec<E>(dtable + (long long)fkey[g] * a.D, a.D, v);
+                    store_row<E>(dtable + (long long)fkey[g] * a.D, a.D, v);
                 }
                 open = false;
             }
@@ -496,7 +510,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
             for (int k = 0; k < E::V; ++k) v[k] += sh[k * 256 + (g << a.lsh) + lane];
 #pragma unroll
         for (int k = 0; k < E::V; ++k) v[k] *= a.scale;
-        store_vec<E>((typename E::T*)a.dtable + (long long)key * a.D + c, a.D, v);
+        store_row<E>((typename E::T*)a.dtable + (long long)key * a.D + c, a.D, v);
     }
 }
 

@@ -237,7 +237,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
             E::unpack(raw[u], v);
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] = act_fwd<ACT>(fmaf(v[k] - mean[k % NG], w[k], b[k]), a.slope);
-            store_vec<E>(y + (long long)r * a.C, W, v);
+            store_tail<E>(y + (long long)r * a.C, dup, W, v);
         }
     }
 }
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
                         const float h = fmaf(v[k], rstd[k % NG], off[k % NG]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                         v[k] = rstd[k % NG] * (w[k] * dz - g1[k % NG] - h * g2[k % NG]);
                     }
-                    store_vec<E>(dx + (long long)r * a.C, W, v);
+                    store_tail<E>(dx + (long long)r * a.C, dup, W, v);
                 }
             }
         }
@@ -386,8 +386,8 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
 struct GnParts {
     int tiles, lc, rows, slots, len, P, tg, llg;    // P: parts a sample; tg: tiles a group may touch
 };
-// The last vector of a row whose width is no multiple of the vector moves back to end with the row: every access is 16 bytes wide, the
-// `dup` elements it shares with the vector before are written twice with the same values and left out of the sums.
+// The last vector of a row whose width is no multiple of the vector moves back to end with the row, so every load is 16 bytes wide; the `dup`
+// elements it shares with the vector before are left out of the sums and the stores.
 struct GnWhere {
     int tile, n, q, rs, c0, W, c, dup, lo, hi;      // c: first channel of the thread's vector
     bool on;
@@ -552,15 +552,62 @@ __global__ __launch_bounds__(256) void gn_stats_join_kernel(GnArgs a, GnParts p,
     }
 }
 
+// The same for the groups of a workgroup's tile, 2^llg lanes each, to LDS: where the parts are few, every workgroup of the second pass joins
+// them itself and a launch is saved.  stat[g - gl] = (mean, 1 / std).
+#define GN_JOIN_GROUPS 512
+template <int V>
+__device__ __forceinline__ int join_here(const GnArgs& a, const GnParts& p, const GnWhere& i, const float4* part, float2* stat) {
+    const int first = a.C < V ? 0 : min(i.c0, a.C - V), gl = first / a.Cg, gh = (i.c0 + i.W - 1) / a.Cg, tw = V << p.lc;
+    const int step = 1 << p.llg, l = threadIdx.x & (step - 1), all = p.P * p.tg;
+    const double inv = 1.0 / ((double)a.S * a.Cg);
+    for (int g = gl + (threadIdx.x >> p.llg); g <= gh; g += 256 >> p.llg) {
+        const int t0 = g * a.Cg / tw, tg = ((g + 1) * a.Cg - 1) / tw - t0 + 1;
+        const float4* mine = part + ((long long)i.n * a.G + g) * all;
+        double total = 0.0, squares = 0.0;
+        for (int q = l; q < all; q += step)
+            if (p.tg == 1 || q % p.tg < tg) total += (double)mine[q].x * mine[q].y;
+        for (int o = step >> 1; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+        const double mean = total * inv;
+        for (int q = l; q < all; q += step)
+            if (p.tg == 1 || q % p.tg < tg) {
+                const float4 o = mine[q];
+                const double d = o.y - mean;
+                squares += o.z + d * d * o.x;
+            }
+        for (int o = step >> 1; o > 0; o >>= 1) squares += __shfl_xor(squares, o, 64);
+        if (l == 0) {
+            const float2 r = make_float2((float)mean, (float)(1.0 / sqrt(squares * inv + (double)a.eps)));
+            stat[g - gl] = r;
+            if (i.q == 0 && t0 == i.tile) {
+                a.mean[i.n * a.G + g] = r.x;
+                a.rstd[i.n * a.G + g] = r.y;
+            }
+        }
+    }
+    __syncthreads();
+    return gl;
+}
+
 template <class E, int ACT, bool NT>
-__global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p) {
+__global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p, const float4* part) {
     constexpr int V = E::V, U = 4;
+    __shared__ float2 stat[GN_JOIN_GROUPS];
     const GnWhere i = where_of<V>(a, p, blockIdx.x);
+    const int gl = part ? join_here<V>(a, p, i, part, stat) : 0;
     if (!i.on) return;
     float mean[V], rstd[V], w[V], b[V];
     load_params<E>(a.w, a.ptype, i.c, a.C, 1.f, w);
     load_params<E>(a.b, a.ptype, i.c, a.C, 0.f, b);
-    load_stats<V>(a, i.n, i.c, mean, rstd);
+    if (part) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float2 st = stat[min(i.c + k, a.C - 1) / a.Cg - gl];
+            mean[k] = st.x;
+            rstd[k] = st.y;
+        }
+    } else {
+        load_stats<V>(a, i.n, i.c, mean, rstd);
+    }
 #pragma unroll
     for (int k = 0; k < V; ++k) w[k] *= rstd[k];
     const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
@@ -577,7 +624,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p) {
                 E::unpack(raw[u], v);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[k] = act_fwd<ACT>(fmaf(v[k] - mean[k], w[k], b[k]), a.slope);
-                store_vec<E, NT>(y + (long long)(r + u * p.rows) * a.C, a.C, v);
+                store_tail<E, NT>(y + (long long)(r + u * p.rows) * a.C, i.dup, a.C, v);
             }
     }
 }
@@ -724,8 +771,8 @@ __device__ __forceinline__ void params_of(const GnArgs& a, int blk, int rows, co
 }
 __global__ __launch_bounds__(256) void gn_params_kernel(GnArgs a, int rows, const float2* ab) { params_of(a, blockIdx.x, rows, ab); }
 
-// dx; the first `pblocks` workgroups sum the parameters' gradients instead.
-template <class E, int ACT, bool NT>
+// dx; the first `pblocks` workgroups sum the parameters' gradients instead.  NT: 1 stores past the caches, 2 loads too.
+template <class E, int ACT, int NT>
 __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef, int pblocks, const float2* ab) {
     constexpr int V = E::V, U = 4;
     if ((int)blockIdx.x < pblocks) {
@@ -749,8 +796,8 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (r + u * p.rows < i.hi) {
-                rx[u] = load_vec<E, NT>(x + (long long)(r + u * p.rows) * a.xr, a.C);
-                rd[u] = load_vec<E, NT>(dy + (long long)(r + u * p.rows) * a.dr, a.C);
+                rx[u] = load_vec<E, NT == 2>(x + (long long)(r + u * p.rows) * a.xr, a.C);
+                rd[u] = load_vec<E, NT == 2>(dy + (long long)(r + u * p.rows) * a.dr, a.C);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -763,7 +810,7 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
                     const float h = fmaf(v[k], rstd[k], off[k]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                     v[k] = rstd[k] * (w[k] * dz - cf[k].x - h * cf[k].y);
                 }
-                store_vec<E, NT>(dx + (long long)(r + u * p.rows) * a.C, a.C, v);
+                store_tail<E, NT != 0>(dx + (long long)(r + u * p.rows) * a.C, i.dup, a.C, v);
             }
     }
 }
@@ -773,7 +820,7 @@ static int vec_of(int dtype) { return dtype == AG2V_F32 ? ElemF32::V : ElemBF16:
 
 // Which way (N, S, C, G) runs, forward or backward.
 struct GnPlan {
-    bool slab, one;
+    bool slab, one, join_here;      // one: a vector lies inside one group; join_here: the second pass joins the parts itself
     GnSlab s;
     int U, threads, blocks, walkers;
     size_t lds;
@@ -792,9 +839,10 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     int kg = 1;
     while (kg < G && (long long)kg * Cg < 8 * V && lcols(kg + 1) <= 3 && ((long long)S << lcols(kg + 1)) <= most) ++kg;
     const int lc = lcols(kg);
-    // narrow rows that are no whole vectors: every cache line would be read by many slabs, in pieces (11 x 4181 x 45 fp32 in 15 groups: 49 us a
-    // training pass; rows of one vector, 8 x 4096 x 256 fp16 in 32 groups, are as fast here, 20.8 us forward, as in parts, 23 us)
-    if (kg < G && Cg % V && (long long)kg * Cg < 4 * V) return false;
+    // narrow rows: every cache line would be read by many slabs, in pieces (13 x 1085 x 1560 fp16 in 195 groups, one vector a row: 147 us a
+    // training pass, 72 us in parts; 11 x 4181 x 45 fp32 in 15 groups, 12 bytes a row: 49 and 37 us).  Forward, rows of whole vectors are no
+    // slower here (8 x 4096 x 256 fp16 in 32 groups: 20.8 us, in parts 22) and take one launch.
+    if (kg < G && (backward ? (long long)kg * Cg < 4 * V : (long long)kg * Cg < 2 * V && Cg % V)) return false;
     if (lc > 10 || ((long long)S << lc) > most) return false;
     const bool one = kg == 1 || Cg % V == 0;
     const int maxT = backward && !one ? 512 : 1024, maxU = backward ? 2 : one ? 8 : 4;
@@ -865,10 +913,19 @@ static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
         r.words = r.coef + 2LL * N * G;
     } else {
         const long long per = ((long long)V << lc) / Cg + 2;
-        p.llg = share_lanes(256, (int)(per < G ? per : G));
+        const long long groups = per < G ? per : G;
+        p.llg = share_lanes(256, (int)groups);
+        r.join_here = groups <= GN_JOIN_GROUPS && groups * p.P * p.tg <= 2048;
         r.words = 4LL * N * G * p.P * p.tg;
     }
     return r;
+}
+
+// Results that go past the caches: large ones whose rows are whole 64-byte pieces.  Others would reach memory in parts of pieces: 10 x 21888 x
+// 150 bf16 forward took 60 us that way and 29 us this way.
+template <class E>
+static bool past_caches(const GnArgs& a) {
+    return (long long)a.N * a.S * a.C * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES && a.C * (long long)sizeof(typename E::T) % 64 == 0;
 }
 
 template <class E, int ACT, bool ONE>
@@ -895,12 +952,16 @@ static int run_fwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) 
     const int blocks = a.N * r.p.P * r.p.tiles;
     hipLaunchKernelGGL(gn_stats_kernel<E>, dim3(blocks), dim3(256), 0, st, a, r.p, (float4*)ws);
     AG2V_CHECK_LAUNCH();
-    hipLaunchKernelGGL(gn_stats_join_kernel<E::V>, dim3(ceil_div((long long)a.N * a.G, 4)), dim3(256), 0, st, a, r.p, (const float4*)ws);
-    AG2V_CHECK_LAUNCH();
-    if ((long long)a.N * a.S * a.C * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES)
-        hipLaunchKernelGGL((gn_apply_kernel<E, ACT, true>), dim3(blocks), dim3(256), 0, st, a, r.p);
+    const float4* part = (const float4*)ws;
+    if (!r.join_here) {
+        hipLaunchKernelGGL(gn_stats_join_kernel<E::V>, dim3(ceil_div((long long)a.N * a.G, 4)), dim3(256), 0, st, a, r.p, part);
+        AG2V_CHECK_LAUNCH();
+        part = nullptr;
+    }
+    if (past_caches<E>(a))
+        hipLaunchKernelGGL((gn_apply_kernel<E, ACT, true>), dim3(blocks), dim3(256), 0, st, a, r.p, part);
     else
-        hipLaunchKernelGGL((gn_apply_kernel<E, ACT, false>), dim3(blocks), dim3(256), 0, st, a, r.p);
+        hipLaunchKernelGGL((gn_apply_kernel<E, ACT, false>), dim3(blocks), dim3(256), 0, st, a, r.p, part);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
@@ -923,10 +984,13 @@ static int run_bwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) 
         AG2V_CHECK_LAUNCH();
         if (a.y) {
             const int pblocks = params ? ceil_div(a.C, 32) : 0;
-            if ((long long)a.N * a.S * a.C * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES)      // x and dy together: the bound of loads
-                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, true>), dim3(blocks + pblocks), dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+            const dim3 grid(blocks + pblocks);
+            if (past_caches<E>(a) && r.p.tiles == 1)      // (x and dy together pass the bound of loads; the lines of a tiled row are read twice)
+                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 2>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+            else if (past_caches<E>(a))
+                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 1>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
             else
-                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, false>), dim3(blocks + pblocks), dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 0>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
             AG2V_CHECK_LAUNCH();
             return AG2V_OK;
         }
