@@ -1,8 +1,8 @@
 // Host side of the fp32 / bf16 / fp16 operators: argument checks, views, workspaces and autograd nodes over the C entry points of
 // include/ag2v.h.  The nodes are C++ because the tape's backward runs on a thread of its own: a node written in Python costs 40 to 100 us
-// there (the interpreter and its objects move between cores), more than the kernels of a small map.  Every refusal is a RuntimeError.
+// there (the interpreter and its objects move between cores), more than the kernels of a small map.  Every refusal of a value is a
+// RuntimeError.
 #include <torch/extension.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -93,18 +93,9 @@ std::tuple<Tensor, int64_t, int64_t> channel_rows(const Tensor& x) {
     return std::make_tuple(x, x.stride(0), row < 0 ? C : row);
 }
 
-// Gradients of a node that has no second derivative: usable, and an error for whoever differentiates them.
-variable_list once(const char* name, variable_list grads) {
-    if (!at::GradMode::is_enabled()) return grads;
-    variable_list some;
-    for (auto& g : grads)
-        if (g.defined()) some.push_back(g.detach().requires_grad_(true));
-    if (some.empty()) return grads;
-    auto wrapped = (*std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative", some.size()))(variable_list(some));
-    size_t k = 0;
-    for (auto& g : grads)
-        if (g.defined()) g = wrapped[k++];
-    return grads;
+// A node without a second derivative: with create_graph=True its gradients would count as constants.
+void first_derivative_only(const char* name) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivative: its backward pass is refused with create_graph=True");
 }
 
 // ---------------------------------------------------------------- embedding
@@ -130,28 +121,22 @@ struct EmbeddingScaled : torch::autograd::Function<EmbeddingScaled> {
         return embed_forward(idx, table, scale);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        first_derivative_only("embedding_scaled");
         const Tensor idx = ctx->get_saved_variables()[0];
         const int64_t V = ctx->saved_data["V"].toInt(), pad = ctx->saved_data["pad"].toInt();
         const double scale = ctx->saved_data["scale"].toDouble();
-        Tensor dtable;
-        {
-            at::NoGradGuard no_grad;
-            const int64_t n = idx.numel(), D = grads[0].size(-1);
-            if (n == 0 || D == 0) {
-                dtable = at::zeros({V, D}, grads[0].options());
-            } else {
-                const auto [dout, sample, ds] = channel_rows(grads[0].unsqueeze(0));
-                const auto [tok, st] = token_rows(idx);
-                dtable = at::empty({V, D}, dout.options());
-                OnDevice on(dout);
-                const int type = elem_of(dout.scalar_type());
-                const size_t floats = lib.embed_bwd_ws(type, n, V, int(D));
-                Tensor ws = workspace_of(dout, floats);
-                checked("ag2v_embed_bwd", lib.embed_bwd(type, tok.data_ptr(), int(tok.element_size()), st, dout.data_ptr(), ds, dtable.data_ptr(), n, V,
-                                                        int(D), float(scale), pad, static_cast<float*>(ptr(ws)), floats, on.stream));
-            }
-        }
-        return once("embedding_scaled", {Tensor(), dtable, Tensor(), Tensor()});
+        const int64_t n = idx.numel(), D = grads[0].size(-1);
+        if (n == 0 || D == 0) return {Tensor(), at::zeros({V, D}, grads[0].options()), Tensor(), Tensor()};
+        const auto [dout, sample, ds] = channel_rows(grads[0].unsqueeze(0));
+        const auto [tok, st] = token_rows(idx);
+        Tensor dtable = at::empty({V, D}, dout.options());
+        OnDevice on(dout);
+        const int type = elem_of(dout.scalar_type());
+        const size_t floats = lib.embed_bwd_ws(type, n, V, int(D));
+        Tensor ws = workspace_of(dout, floats);
+        checked("ag2v_embed_bwd", lib.embed_bwd(type, tok.data_ptr(), int(tok.element_size()), st, dout.data_ptr(), ds, dtable.data_ptr(), n, V, int(D),
+                                                float(scale), pad, static_cast<float*>(ptr(ws)), floats, on.stream));
+        return {Tensor(), dtable, Tensor(), Tensor()};
     }
 };
 
@@ -205,34 +190,33 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        first_derivative_only("group_norm_act");
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+        const bool some = x.numel() > 0;
+        const auto made = [&](const Tensor& like) {
+            return some ? at::empty(like.sizes(), like.options().memory_format(at::MemoryFormat::Contiguous)) : at::zeros(like.sizes(), like.options());
+        };
         Tensor dx, dw, db;
-        {
-            at::NoGradGuard no_grad;
-            const bool some = x.numel() > 0;
-            const auto made = [&](const Tensor& like) { return some ? at::empty(like.sizes(), like.options().memory_format(at::MemoryFormat::Contiguous))
-                                                                    : at::zeros(like.sizes(), like.options()); };
-            if (ctx->needs_input_grad(0)) dx = made(x);
-            // (the edges are those of the tensors that are there)
-            if (weight.defined() && ctx->needs_input_grad(1)) dw = made(weight);
-            if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) db = made(bias);
-            if (some) {
-                const int64_t N = x.size(0), C = x.size(-1), S = positions(x), groups = stats.size(2);
-                const auto [xrows, xs, xr] = channel_rows(x);
-                const auto [drows, ds, dr] = channel_rows(grads[0]);
-                OnDevice on(x);
-                const int type = elem_of(x.scalar_type());
-                const size_t floats = lib.norm_ws(type, int(N), int(S), int(C), int(groups), 1);
-                Tensor ws = workspace_of(x, floats);
-                const float* mean = stats.data_ptr<float>();
-                checked("ag2v_group_norm_bwd", lib.norm_bwd(type, drows.data_ptr(), ds, dr, xrows.data_ptr(), xs, xr, ptr(weight), ptr(bias),
-                                                            param_type(weight, bias), mean, mean + N * groups, ptr(dx), ptr(dw), ptr(db), int(N), int(S),
-                                                            int(C), int(groups), int(ctx->saved_data["act"].toInt()),
-                                                            float(ctx->saved_data["slope"].toDouble()), static_cast<float*>(ptr(ws)), floats, on.stream));
-            }
+        if (ctx->needs_input_grad(0)) dx = made(x);
+        // (the edges are those of the tensors that are there)
+        if (weight.defined() && ctx->needs_input_grad(1)) dw = made(weight);
+        if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) db = made(bias);
+        if (some) {
+            const int64_t N = x.size(0), C = x.size(-1), S = positions(x), groups = stats.size(2);
+            const auto [xrows, xs, xr] = channel_rows(x);
+            const auto [drows, ds, dr] = channel_rows(grads[0]);
+            OnDevice on(x);
+            const int type = elem_of(x.scalar_type());
+            const size_t floats = lib.norm_ws(type, int(N), int(S), int(C), int(groups), 1);
+            Tensor ws = workspace_of(x, floats);
+            const float* mean = stats.data_ptr<float>();
+            checked("ag2v_group_norm_bwd", lib.norm_bwd(type, drows.data_ptr(), ds, dr, xrows.data_ptr(), xs, xr, ptr(weight), ptr(bias),
+                                                        param_type(weight, bias), mean, mean + N * groups, ptr(dx), ptr(dw), ptr(db), int(N), int(S), int(C),
+                                                        int(groups), int(ctx->saved_data["act"].toInt()), float(ctx->saved_data["slope"].toDouble()),
+                                                        static_cast<float*>(ptr(ws)), floats, on.stream));
         }
-        return once("group_norm_act", {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()});
+        return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 

@@ -64,6 +64,30 @@ def test_embedding_scaled(n, V, D, kind, dtype, device):
     _embed_case(device, idx, _randn(V, D, seed=1, dtype=dtype), 0.37, None, _randn(n, D, seed=2, scale=0.1, dtype=dtype), 'embed')
 
 
+# sizes at which the gradient changes its way: one launch, counted ranks, one radix pass, several, several rounds a workgroup
+@pytest.mark.parametrize("n,V,D,kind", [(1024, 4, 300, 'skewed'), (1025, 4, 300, 'skewed'), (2048, 30, 128, 'one'), (2049, 30, 128, 'one'), (2048, 1100, 3, 'cyclic'),
+                                        (6144, 511, 20, 'skewed'), (6145, 511, 20, 'skewed'), (6145, 512, 20, 'skewed'), (262144, 40, 8, 'skewed'),
+                                        (262145, 700, 4, 'skewed'), (300001, 300000, 2, 'uniform')], ids=str)
+def test_embedding_scaled_switching_sizes(n, V, D, kind, device):
+    idx = _tokens(n, V, n, kind)
+    for dtype in (torch.float32, torch.float16):
+        _embed_case(device, idx, _randn(V, D, seed=1, dtype=dtype), 1.0, V // 3, _randn(n, D, seed=2, scale=0.1, dtype=dtype), 'embed')
+
+
+def test_embedding_scaled_past_the_caches(device):
+    """Results and gradients large enough to go past the caches.  Whole numbers: every product and sum is exact."""
+    from ag2video_amd import ops
+    g = torch.Generator(device=device).manual_seed(0)
+    for n, V, D in ((140001, 60000, 133), (80000, 70000, 130)):
+        idx = torch.randint(V, (n,), device=device, generator=g)
+        table = torch.randint(-50, 50, (V, D), device=device, generator=g).float().requires_grad_(True)
+        dout = torch.randint(-50, 50, (n, D), device=device, generator=g).float()
+        out = ops.embedding_scaled(idx, table, 2.0)
+        assert torch.equal(out, table.detach()[idx] * 2)
+        (grad,) = torch.autograd.grad(out, table, dout)
+        assert torch.equal(grad, torch.zeros(V, D, device=device, dtype=torch.float64).index_add_(0, idx, dout.double()).float() * 2)
+
+
 @pytest.mark.parametrize("pad", [None, 0, 11], ids=str)
 @pytest.mark.parametrize("shape", [(), (5,), (3, 4), (2, 3, 50), (0,), (4, 0)], ids=str)
 def test_embedding_scaled_shapes_and_padding(shape, pad, device):
@@ -200,6 +224,46 @@ def test_group_norm_act_forms(act, affine, dtype, device):
     for shape, groups in (((2, 50, 24), 3), ((2, 3000, 36), 4), ((2, 9, 10), 2)):
         _norm_case(device, shape, groups, dtype, act, affine, dtype, seed=7)
         _norm_case(device, shape, groups, dtype, act, affine, torch.float32, seed=9, eps=0.1, slope=0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("S", [1024, 1025, 2047, 2049, 4096, 4097, 8193], ids=str)
+def test_group_norm_act_switching_sizes(S, dtype, device):
+    """Positions at which slabs get narrower or parts take over, in groups of whole vectors, of odd widths, and of all channels."""
+    for C, G in ((64, 8), (44, 4), (15, 5), (24, 1)):
+        _norm_case(device, (1, S, C), G, dtype, 'silu', True, torch.float32, seed=S)
+
+
+@pytest.mark.parametrize("C,G", [(2312, 1), (2312, 2312), (1156, 4), (1200, 75)], ids=str)
+def test_group_norm_act_wide(C, G, device):
+    """Several tiles a row; groups of many tiles and many groups a tile."""
+    for dtype in (torch.float32, torch.bfloat16):
+        _norm_case(device, (2, 300, C), G, dtype, 'lrelu', True, torch.float32, seed=C)
+        _norm_case(device, (1, 2600, C), G, dtype, 'silu', True, dtype, seed=G)
+
+
+@pytest.mark.parametrize("C", [64, 90, 112], ids=str)
+def test_group_norm_act_batch_does_not_matter(C, device):
+    """y and dx of a sample are the same bits alone and in a batch, also where only the batch is large enough to go past the caches."""
+    from ag2video_amd import ops
+    N, S = 3, 72000
+    x = torch.randn(N, S, C, device=device, generator=torch.Generator(device=device).manual_seed(1))
+    dy = torch.randn(N, S, C, device=device, generator=torch.Generator(device=device).manual_seed(2))
+    w, b = _randn(C, seed=3).to(device), _randn(C, seed=4).to(device)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = ops.group_norm_act(leaves[0], 2, *leaves[1:])
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    sums, mags = torch.zeros(2, C, device=device, dtype=torch.float64), torch.zeros(2, C, device=device, dtype=torch.float64)
+    for n in range(N):
+        one = [t.clone().requires_grad_(True) for t in (x[n:n + 1], w, b)]
+        y1 = ops.group_norm_act(one[0], 2, *one[1:])
+        dx1, *dp = torch.autograd.grad(y1, one, dy[n:n + 1])
+        assert torch.equal(y1[0], y[n]) and torch.equal(dx1[0], dx[n])
+        dp = torch.stack(dp).double()
+        sums += dp
+        mags += dp.abs()
+    # the parameters' gradients are the samples' own, joined by two fp32 additions of at most the magnitudes' sum each
+    assert ((torch.stack((dw, db)).double() - sums).abs() <= 2 * R.U * mags).all()
 
 
 def test_group_norm_act_far_mean(device):
@@ -506,8 +570,29 @@ def test_modules(device):
 
 
 def test_no_second_derivative(device):
+    """Differentiating a gradient is an error and not a wrong number: the backward pass is refused where its graph is asked for."""
     from ag2video_amd import ops
     x = torch.randn(2, 5, 8, device=device, requires_grad=True)
-    (g,) = torch.autograd.grad(ops.group_norm_act(x, 2).sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(g.sum(), x)
+    table = torch.randn(6, 8, device=device, requires_grad=True)
+    for leaf, y in ((x, ops.group_norm_act(x, 2)), (table, ops.embedding_scaled(torch.arange(4, device=device), table))):
+        with pytest.raises(RuntimeError, match='second derivative'):
+            torch.autograd.grad(y.square().sum(), leaf, create_graph=True)
+
+
+def test_refusals(device):
+    """What the operators refuse of tensors on the device."""
+    from ag2video_amd import ops
+    idx, table = torch.zeros(3, dtype=torch.long, device=device), torch.zeros(4, 8, device=device)
+    x = torch.zeros(2, 3, 8, device=device)
+    for call in (lambda: ops.embedding_scaled(idx.cpu(), table), lambda: ops.embedding_scaled(idx.float(), table), lambda: ops.embedding_scaled(idx.short(), table),
+                 lambda: ops.embedding_scaled(idx, table.double()), lambda: ops.embedding_scaled(idx, table[0]), lambda: ops.embedding_scaled(idx, table[:0]),
+                 lambda: ops.embedding_scaled(idx, table, 1.0, 4), lambda: ops.embedding_scaled(idx, table, 1.0, -1), lambda: ops.embedding_scaled(idx, table.long()),
+                 lambda: ops.group_norm_act(x, 3), lambda: ops.group_norm_act(x, 0), lambda: ops.group_norm_act(x, -2), lambda: ops.group_norm_act(x[0, 0], 2),
+                 lambda: ops.group_norm_act(x.double(), 2), lambda: ops.group_norm_act(x, 2, act='tanh'), lambda: ops.group_norm_act(x, 2, eps=-1.0),
+                 lambda: ops.group_norm_act(x, 2, eps=float('nan')), lambda: ops.group_norm_act(x, 2, slope=float('nan')),
+                 lambda: ops.group_norm_act(x, 2, torch.ones(7, device=device)), lambda: ops.group_norm_act(x, 2, torch.ones(8)),
+                 lambda: ops.group_norm_act(x, 2, None, torch.ones(8, 1, device=device)), lambda: ops.group_norm_act(x, 2, torch.ones(8, device=device).half()),
+                 lambda: ops.group_norm_act(x.half(), 2, torch.ones(8, device=device), torch.ones(8, device=device).half()),
+                 lambda: ops.group_norm_act(x[..., :0], 1), lambda: ops.group_norm_act(torch.zeros(1, device=device).expand(1 << 22, 1, 8), 8)):
+        with pytest.raises(RuntimeError):
+            call()
