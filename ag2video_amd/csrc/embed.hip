@@ -8,10 +8,12 @@
 //
 // The gradient, by sizes:
 //   few rows, few tokens    one launch: a workgroup per row of the table picks its tokens out of all n (embed_pick_kernel);
+//   few rows                one workgroup sorts a tile of tokens in LDS and sums its rows by token; a second launch adds the tiles' sums
+//                           (embed_tile_kernel, embed_tile_join_kernel);
 //   up to RANK_MAX tokens   a token's place in the sorted order is the number of tokens before it: n^2 compares, spread over the whole
 //                           chip in ONE launch that also clears the table's gradient (embed_rank_kernel);
 //   more                    a stable radix sort, 9 bits a pass, two launches a pass (embed_hist_kernel, embed_scatter_kernel).
-// After a sort, embed_sum_kernel walks equal shares of the sorted order -- a long run of one token costs no more than many short ones --
+// After a sort of all tokens, embed_sum_kernel walks equal shares of the sorted order -- a long run of one token costs no more than many short ones --
 // and writes every row whose tokens lie inside one workgroup's share; embed_join_kernel adds the rest up, in order.  No atomics on
 // floating-point values: equal calls give equal bits.
 #include "elem.h"
@@ -37,6 +39,24 @@ __device__ __forceinline__ void store_row(typename E::T* p, int width, const flo
         asm volatile("" : "+v"(v[k]));
     }
     store_vec<E, NT>(p, width, v);
+}
+
+// acc of group 0 += acc of all other groups of 2^lsh lanes, pairwise; sh: V floats a thread.  All threads of the workgroup.
+template <int V, int THREADS>
+__device__ __forceinline__ void join_groups(float (&acc)[V], float* sh, int lsh) {
+    const int grp = threadIdx.x >> lsh;
+#pragma unroll
+    for (int k = 0; k < V; ++k) sh[k * THREADS + threadIdx.x] = acc[k];
+    for (int o = (THREADS >> lsh) >> 1; o > 0; o >>= 1) {
+        __syncthreads();
+        if (grp < o) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                acc[k] += sh[k * THREADS + threadIdx.x + (o << lsh)];
+                sh[k * THREADS + threadIdx.x] = acc[k];
+            }
+        }
+    }
 }
 
 // ---------------------------------------------------------------- lookup
@@ -127,16 +147,221 @@ __global__ __launch_bounds__(PICK_THREADS) void embed_pick_kernel(const void* __
                     for (int k = 0; k < E::V; ++k) acc[k] += x[k];
                 }
         }
-#pragma unroll
-    for (int k = 0; k < E::V; ++k) part[k * PICK_THREADS + threadIdx.x] = acc[k];
-    __syncthreads();
+    join_groups<E::V, PICK_THREADS>(acc, part, lsh);
     if (grp == 0 && c0 < D) {
-        for (int g = 1; g * share < total; ++g)
-#pragma unroll
-            for (int k = 0; k < E::V; ++k) acc[k] += part[k * PICK_THREADS + (g << lsh) + lane];
 #pragma unroll
         for (int k = 0; k < E::V; ++k) acc[k] *= scale;
         store_row<E>(dtable + (long long)v * D + c, D, acc);
+    }
+}
+
+// V of the D floats at p
+template <int V>
+__device__ __forceinline__ void load_part(const float* p, int D, float (&v)[V]) {
+    if (D >= V) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            const u32x4 r = *reinterpret_cast<const u32x4_a4*>(p + k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[k + j] = __uint_as_float(r[j]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = k < D ? p[k] : 0.f;
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_part(float* p, int D, const float (&v)[V]) {
+    if (D >= V) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            u32x4 r;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = __float_as_uint(v[k + j]);
+            *reinterpret_cast<u32x4_a4*>(p + k) = r;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (k < D) p[k] = v[k];
+    }
+}
+
+// ---------------------------------------------------------------- gradient: tiles of tokens, for few rows
+// A workgroup sorts T tokens by counting (ranks within a wave by matching the keys' bits over ballots, then over waves), its groups of lanes
+// walk equal shares of the sorted tile as in embed_sum_kernel below, and the sum of each token that occurs goes to part[tile][token][:],
+// count[tile][token] says how often it does.  No pass over the tokens but this one.
+#define TILE_THREADS 512
+#define TILE_MIN 512
+#define TILE_MAX 2048
+#define TILE_BITS 9
+struct TileArgs {
+    const void *idx, *dout;
+    void* dtable;
+    int* count;
+    float* part;
+    long long istride, dstride;
+    int wide, n, V, D, pad, lsh, T, bits, tiles;
+    float scale;
+};
+template <class E, bool NT>
+__global__ __launch_bounds__(TILE_THREADS) void embed_tile_kernel(TileArgs a) {
+    constexpr int U = 8, PER = TILE_MAX / TILE_THREADS, W = TILE_THREADS / 64, DIG = 1 << TILE_BITS;
+    static_assert(DIG == TILE_THREADS, "a thread scans one key");
+    __shared__ int cnt[W][DIG], wsum[W], flags[TILE_THREADS / 8];
+    __shared__ unsigned short skey[TILE_MAX], spos[TILE_MAX];
+    __shared__ float head[TILE_THREADS * E::V];
+    const int tile = blockIdx.x % a.tiles, slice = blockIdx.x / a.tiles, t0 = tile * a.T;
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, rounds = a.T / TILE_THREADS, own = a.T / W;
+#pragma unroll
+    for (int w = 0; w < W; ++w) cnt[w][threadIdx.x] = 0;
+    int key[PER], rank[PER];
+#pragma unroll
+    for (int q = 0; q < PER; ++q)
+        if (q < rounds) {
+            const int i = t0 + wave * own + q * 64 + wl;
+            key[q] = i < a.n ? key_at(a.idx, a.wide, a.istride, i, a.V, a.pad) : a.V;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < PER; ++q)
+        if (q < rounds) {
+            unsigned long long m = ~0ull;
+            for (int b = 0; b < a.bits; ++b) {
+                const bool bit = (key[q] >> b) & 1;
+                const unsigned long long same = __ballot(bit);
+                m &= bit ? same : ~same;
+            }
+            const int lower = __popcll(m & ((1ull << wl) - 1)), seen = cnt[wave][key[q]];
+            __builtin_amdgcn_wave_barrier();
+            if (lower == 0) cnt[wave][key[q]] = seen + __popcll(m);
+            __builtin_amdgcn_wave_barrier();
+            rank[q] = seen + lower;
+        }
+    __syncthreads();
+    // exclusive sums over keys, then waves
+    {
+        const int d = threadIdx.x;
+        int c[W], all = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            c[w] = cnt[w][d];
+            all += c[w];
+        }
+        if (slice == 0 && d < a.V) a.count[tile * a.V + d] = all;
+        int scan = all;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(scan, o, 64);
+            if (wl >= o) scan += up;
+        }
+        if (wl == 63) wsum[wave] = scan;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) scan += wsum[w];
+        int run = scan - all;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            cnt[w][d] = run;
+            run += c[w];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < PER; ++q)
+        if (q < rounds) {
+            const int at = cnt[wave][key[q]] + rank[q];
+            skey[at] = (unsigned short)key[q];
+            spos[at] = (unsigned short)(wave * own + q * 64 + wl);
+        }
+    __syncthreads();
+    const int lane = threadIdx.x & ((1 << a.lsh) - 1), grp = threadIdx.x >> a.lsh, ng = TILE_THREADS >> a.lsh, L = a.T / ng;
+    const int c0 = ((slice << a.lsh) + lane) * E::V, c = a.D < E::V ? 0 : min(c0, a.D - E::V);
+    const bool mine = c0 < a.D;
+    const typename E::T* dout = (const typename E::T*)a.dout + (long long)t0 * a.dstride + c;
+    float* part = a.part + (long long)tile * a.V * a.D + c;
+    const int e0 = grp * L, e1 = e0 + L;
+    int cur = skey[e0], flag = e0 > 0 && skey[e0 - 1] == cur ? 1 : 0;      // (see embed_sum_kernel)
+    bool began_before = flag;
+    const int next = e1 < a.T ? skey[e1] : -1;
+    float acc[E::V] = {};
+    const auto finish = [&]() {
+        if (began_before) {
+#pragma unroll
+            for (int k = 0; k < E::V; ++k) head[k * TILE_THREADS + threadIdx.x] = acc[k];
+        } else if (cur != a.V && mine) {
+            store_part<E::V>(part + (long long)cur * a.D, a.D, acc);
+        }
+    };
+    for (int e = e0; e < e1; e += U) {
+        int k8[U];
+        u32x4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            k8[u] = skey[e + u];
+            if (k8[u] != a.V && mine) r[u] = load_vec<E, NT>(dout + spos[e + u] * a.dstride, a.D);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k8[u] != cur) {
+                finish();
+                cur = k8[u];
+                began_before = false;
+#pragma unroll
+                for (int k = 0; k < E::V; ++k) acc[k] = 0.f;
+            }
+            if (k8[u] != a.V && mine) {
+                float x[E::V];
+                E::unpack(r[u], x);
+#pragma unroll
+                for (int k = 0; k < E::V; ++k) acc[k] += x[k];
+            }
+        }
+    }
+    if (next != cur || began_before) finish();
+    if (next == cur) flag |= began_before ? 2 : 4;
+    if (lane == 0) flags[grp] = flag;
+    __syncthreads();
+    if ((flag & 4) && cur != a.V && mine) {
+        for (int g = grp + 1; g < ng; ++g) {
+#pragma unroll
+            for (int k = 0; k < E::V; ++k) acc[k] += head[k * TILE_THREADS + (g << a.lsh) + lane];
+            if (!(flags[g] & 2)) break;
+        }
+        store_part<E::V>(part + (long long)cur * a.D, a.D, acc);
+    }
+}
+
+// dtable[v] = scale * the tiles' sums of token v, in order: 2^lsh lanes a column share, the tiles shared over the groups.
+template <class E>
+__global__ __launch_bounds__(PICK_THREADS) void embed_tile_join_kernel(TileArgs a) {
+    constexpr int U = 8;
+    __shared__ float sh[PICK_THREADS * E::V];
+    const int v = blockIdx.x % a.V, slice = blockIdx.x / a.V;
+    const int lane = threadIdx.x & ((1 << a.lsh) - 1), grp = threadIdx.x >> a.lsh, ng = PICK_THREADS >> a.lsh;
+    const int c0 = ((slice << a.lsh) + lane) * E::V, c = a.D < E::V ? 0 : min(c0, a.D - E::V);
+    const int share = (a.tiles + ng - 1) / ng, q1 = min(a.tiles, (grp + 1) * share);
+    float acc[E::V] = {};
+    if (c0 < a.D)
+        for (int q = grp * share; q < q1; q += U) {
+            bool in[U];
+            float x[U][E::V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) in[u] = q + u < q1 && a.count[(q + u) * a.V + v] > 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (in[u]) load_part<E::V>(a.part + ((long long)(q + u) * a.V + v) * a.D + c, a.D, x[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (in[u]) {
+#pragma unroll
+                    for (int k = 0; k < E::V; ++k) acc[k] += x[u][k];
+                }
+        }
+    join_groups<E::V, PICK_THREADS>(acc, sh, a.lsh);
+    if (grp == 0 && c0 < a.D) {
+#pragma unroll
+        for (int k = 0; k < E::V; ++k) acc[k] *= a.scale;
+        store_row<E>((typename E::T*)a.dtable + (long long)v * a.D + c, a.D, acc);
     }
 }
 
@@ -321,8 +546,9 @@ __global__ __launch_bounds__(RADIX_THREADS) void embed_scatter_kernel(RadixSrc s
 
 // ---------------------------------------------------------------- gradient: sums over the sorted order
 // A group of 2^lsh lanes walks L sorted entries, eight rows in flight.  A segment (the entries of one token) that begins and ends in its
-// share goes to the table at once; the part of one that began earlier (head) or goes on (tail) goes to LDS, where one group joins them in
-// order; what began before the workgroup or goes on behind it goes to part[0 / 1][workgroup][:] for embed_join_kernel.
+// share goes to the table at once.  The end of one that began earlier goes to LDS (head), and the group where a segment begins and goes on
+// adds the heads behind its own part.  flags: 1 the share begins inside a segment, 2 which fills it and goes on, 4 a segment begins in the
+// share and goes on.  What began before the workgroup or goes on behind it goes to part[0 / 1][workgroup][:] for embed_join_kernel.
 struct SumArgs {
     const int *skey, *order;
     const void* dout;
@@ -335,8 +561,8 @@ struct SumArgs {
 template <class E, bool NT>
 __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
     constexpr int U = 8;
-    __shared__ float head[256 * E::V], tail[256 * E::V];
-    __shared__ int flags[32], fkey[32], lkey[32];
+    __shared__ float head[256 * E::V];
+    __shared__ int flags[32];
     const int lane = threadIdx.x & ((1 << a.lsh) - 1), grp = threadIdx.x >> a.lsh, ng = 256 >> a.lsh;
     const int blk = blockIdx.x % a.nblk, slice = blockIdx.x / a.nblk;
     const int c0 = ((slice << a.lsh) + lane) * E::V, c = a.D < E::V ? 0 : min(c0, a.D - E::V);
@@ -344,14 +570,14 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
     const typename E::T* dout = (const typename E::T*)a.dout + c;
     typename E::T* dtable = (typename E::T*)a.dtable + c;
     const long long e0 = ((long long)blk * ng + grp) * a.L, e1 = min((long long)a.n, e0 + a.L);
+    int cur = a.V, flag = 0;
+    float acc[E::V] = {};
     if (e0 < e1) {
-        int cur = a.skey[e0];
-        const int first = cur;
+        cur = a.skey[e0];
         bool began_before = e0 > 0 && a.skey[e0 - 1] == cur;
         const int next = e1 < a.n ? a.skey[e1] : -1;
-        int f = began_before ? 1 : 0;
-        float acc[E::V] = {};
-        auto finish = [&]() {          // the segment `cur` ends here
+        flag = began_before ? 1 : 0;
+        const auto finish = [&]() {          // the segment `cur` ends here, or the share does
             if (began_before) {
 #pragma unroll
                 for (int k = 0; k < E::V; ++k) head[k * 256 + threadIdx.x] = acc[k];
@@ -392,73 +618,35 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
                     }
                 }
         }
-        if (next != cur) {
-            finish();
-        } else if (began_before) {     // one segment fills the share and goes on
-            f |= 2;
-#pragma unroll
-            for (int k = 0; k < E::V; ++k) head[k * 256 + threadIdx.x] = acc[k];
-        } else {
-            f |= 4;
-#pragma unroll
-            for (int k = 0; k < E::V; ++k) tail[k * 256 + threadIdx.x] = acc[k];
-        }
-        if (lane == 0) { flags[grp] = f; fkey[grp] = first; lkey[grp] = cur; }
-    } else if (lane == 0) {
-        flags[grp] = 0;
+        if (next != cur || began_before) finish();
+        if (next == cur) flag |= began_before ? 2 : 4;
     }
+    if (lane == 0) flags[grp] = flag;
     __syncthreads();
-    if (grp != 0 || !mine) return;
-    float acc[E::V] = {};
-    bool open = false, outside = false;
+    if (!mine) return;
     float* part = a.part + (long long)blk * a.D + c;
-    const long long half = (long long)a.nblk * a.D;
-    auto spill = [&](float* to) {
+    // group g's head onto x; whether the segment goes on behind it
+    const auto add_head = [&](float (&x)[E::V], int g) {
 #pragma unroll
-        for (int k = 0; k < E::V; ++k)
-            if (k < a.D) to[k] = acc[k];
+        for (int k = 0; k < E::V; ++k) x[k] += head[k * 256 + (g << a.lsh) + lane];
+        return (flags[g] & 2) != 0;
     };
-    for (int g = 0; g < ng; ++g) {
-        const int f = flags[g], at = (g << a.lsh) + lane;
-        if (f & 1) {
-            if (!open) { open = outside = true; }
+    if (flag & 4) {
+        bool open = true;
+        for (int g = grp + 1; open && g < ng; ++g) open = add_head(acc, g);
+        if (open) {
+            store_part<E::V>(part + (long long)a.nblk * a.D, a.D, acc);
+        } else if (cur != a.V) {
 #pragma unroll
-            for (int k = 0; k < E::V; ++k) acc[k] += head[k * 256 + at];
-            if (!(f & 2)) {
-                if (outside) {
-                    spill(part);
-                } else if (fkey[g] != a.V) {
-                    float v[E::V];
-#pragma unroll
-                    for (int k = 0; k < E::V; ++k) v[k] = acc[k] * a.scale;
-                    store_row<E>(dtable + (long long)fkey[g] * a.D, a.D, v);
-                }
-                open = false;
-            }
-        }
-        if (f & 4) {
-            open = true;
-            outside = false;
-#pragma unroll
-            for (int k = 0; k < E::V; ++k) acc[k] = tail[k * 256 + at];
+            for (int k = 0; k < E::V; ++k) acc[k] *= a.scale;
+            store_row<E>(dtable + (long long)cur * a.D, a.D, acc);
         }
     }
-    if (open) spill(outside ? part : part + half);
-}
-
-// V of the D floats at p
-template <int V>
-__device__ __forceinline__ void load_part(const float* p, int D, float (&v)[V]) {
-    if (D >= V) {
-#pragma unroll
-        for (int k = 0; k < V; k += 4) {
-            const u32x4 r = *reinterpret_cast<const u32x4_a4*>(p + k);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[k + j] = __uint_as_float(r[j]);
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = k < D ? p[k] : 0.f;
+    if (grp == 0 && (flag & 1)) {
+        float x[E::V] = {};
+        bool open = true;
+        for (int g = 0; open && g < ng; ++g) open = add_head(x, g);
+        store_part<E::V>(part, a.D, x);
     }
 }
 
@@ -496,20 +684,13 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
                 }
         }
     }
-#pragma unroll
-    for (int k = 0; k < E::V; ++k) sh[k * 256 + threadIdx.x] = acc[k];
-    __syncthreads();
+    join_groups<E::V, 256>(acc, sh, a.lsh);
     if (grp == 0 && c0 < a.D) {
         const float* tail = a.part + (long long)a.nblk * a.D + (long long)blk * a.D + c;
         float v[E::V];
         load_part<E::V>(tail, a.D, v);
 #pragma unroll
-        for (int k = 0; k < E::V; ++k) v[k] += acc[k];
-        for (int g = 1; g < ng; ++g)
-#pragma unroll
-            for (int k = 0; k < E::V; ++k) v[k] += sh[k * 256 + (g << a.lsh) + lane];
-#pragma unroll
-        for (int k = 0; k < E::V; ++k) v[k] *= a.scale;
+        for (int k = 0; k < E::V; ++k) v[k] = (v[k] + acc[k]) * a.scale;
         store_row<E>((typename E::T*)a.dtable + (long long)key * a.D + c, a.D, v);
     }
 }
@@ -527,9 +708,9 @@ static int vec_of(int dtype) { return dtype == AG2V_F32 ? ElemF32::V : ElemBF16:
 
 // How the gradient of (n, V, D) runs.
 struct EmbedPlan {
-    bool pick, rank;
+    bool pick, tile, rank;
     int lsh, slices, L, nblk;       // sums
-    int passes, bits, rounds, nb;   // radix
+    int T, tiles, bits, passes, rounds, nb;   // tiles; radix
     long long npad, words;          // workspace: sorted keys and positions, their ping-pong, counts, parts
 };
 static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
@@ -541,6 +722,21 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
     // one workgroup may get all n tokens: at most 64 rows a group of lanes then
     p.pick = n <= 64LL * (PICK_THREADS >> p.lsh) && n <= PICK_MAX && V * p.slices <= 1024;
     if (p.pick) return p;
+    // about 256 tiles, at most 512, whose sums (fp32, V rows a tile) are at most a quarter of the bytes of the rows summed: 131072 tokens of 27
+    // words, 128 wide, take 23 us so and 33 us by a radix pass; 524288 of 256 words in fp16, half the rows' bytes, 72 and 55 us
+    p.T = TILE_MIN;
+    while (p.T < TILE_MAX && n >= 512LL * p.T) p.T *= 2;
+    p.tile = V * 16 <= (dtype == AG2V_F32 ? 4 : 2) * p.T && n <= 512LL * TILE_MAX;
+    if (p.tile) {
+        if (p.lsh > 4) {                // 16 lanes a row: shares of 16 tokens at least, and more workgroups
+            p.lsh = 4;
+            p.slices = (int)((cv + 15) >> 4);
+        }
+        p.tiles = (int)((n + p.T - 1) / p.T);
+        p.bits = log2_up(V + 1);
+        p.words = ((long long)p.tiles * V + 3) / 4 * 4 + (long long)p.tiles * V * D;
+        return p;
+    }
     // counting takes 6.2 us for 2156 tokens, 10.5 for 5849, 25 for 11925; a radix pass 12: one pass (V < 512) is faster from 6000 tokens on,
     // two or more from about 11000
     p.rank = n <= (V < RADIX_N ? RANK_MAX * 3 / 4 : RANK_MAX);
@@ -588,6 +784,19 @@ static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istr
     if (p.pick) {
         hipLaunchKernelGGL(embed_pick_kernel<E>, dim3(V * p.slices), dim3(PICK_THREADS), 0, st, idx, wide, istride, (const typename E::T*)dout, dstride,
                            (typename E::T*)dtable, n, V, D, scale, pad, p.lsh);
+        AG2V_CHECK_LAUNCH();
+        return AG2V_OK;
+    }
+    if (p.tile) {
+        int* count = (int*)workspace;
+        const TileArgs t = {idx, dout, dtable, count, workspace + ((long long)p.tiles * V + 3) / 4 * 4, istride, dstride, wide, n, V, D, pad, p.lsh, p.T, p.bits,
+                            p.tiles, scale};
+        if ((long long)n * D * (long long)sizeof(typename E::T) > AG2V_NT_LOAD_BYTES)
+            hipLaunchKernelGGL((embed_tile_kernel<E, true>), dim3(p.tiles * p.slices), dim3(TILE_THREADS), 0, st, t);
+        else
+            hipLaunchKernelGGL((embed_tile_kernel<E, false>), dim3(p.tiles * p.slices), dim3(TILE_THREADS), 0, st, t);
+        AG2V_CHECK_LAUNCH();
+        hipLaunchKernelGGL(embed_tile_join_kernel<E>, dim3(V * p.slices), dim3(PICK_THREADS), 0, st, t);
         AG2V_CHECK_LAUNCH();
         return AG2V_OK;
     }
