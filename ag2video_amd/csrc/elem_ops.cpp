@@ -146,8 +146,8 @@ Tensor embedding_scaled(const Tensor& idx, Tensor table, double scale, std::opti
     TORCH_CHECK(idx.scalar_type() == at::kInt || idx.scalar_type() == at::kLong, "embedding_scaled: expected int32 or int64 tokens, got ",
                 idx.scalar_type());
     TORCH_CHECK(idx.device() == table.device(), "embedding_scaled: tokens on ", idx.device(), ", table on ", table.device());
-    TORCH_CHECK(idx.numel() < INT_LIMIT && table.size(0) < INT_LIMIT - 1 && table.size(1) < INT_LIMIT, "embedding_scaled: ", idx.numel(),
-                " tokens, table ", table.sizes(), ": fewer than 2^31 of each");
+    TORCH_CHECK(idx.numel() < INT_LIMIT && table.size(0) < INT_LIMIT - 1 && table.size(1) < INT_LIMIT / 2, "embedding_scaled: ", idx.numel(),
+                " tokens, table ", table.sizes(), ": fewer than 2^31 tokens and rows, 2^30 columns");
     TORCH_CHECK(!padding_idx || (*padding_idx >= 0 && *padding_idx < table.size(0)), "embedding_scaled: padding_idx ", padding_idx.value_or(0),
                 " outside [0, ", table.size(0), ")");
     if ((table.size(1) > 1 && table.stride(1) != 1) || table.stride(0) < table.size(1)) table = table.contiguous();
@@ -230,8 +230,8 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const std::optional<Tenso
     const int64_t code = act == "silu" ? 1 : act == "lrelu" ? 2 : act == "none" ? 0 : -1;
     TORCH_CHECK(code >= 0, name, ": unknown activation '", act, "' (silu, lrelu, none)");
     TORCH_CHECK(eps >= 0 && eps < std::numeric_limits<double>::infinity() && !std::isnan(slope), name, ": eps ", eps, ", slope ", slope);
-    TORCH_CHECK(N * groups < (int64_t(1) << 24) && positions(x) < INT_LIMIT && C < INT_LIMIT, name, ": ", x.sizes(), " in ", groups,
-                " groups: fewer than 2^24 (sample, group) pairs, 2^31 positions and channels");
+    TORCH_CHECK(N * groups < (int64_t(1) << 24) && positions(x) < INT_LIMIT / 2 && C < INT_LIMIT / 2, name, ": ", x.sizes(), " in ", groups,
+                " groups: fewer than 2^24 (sample, group) pairs, 2^30 positions and channels");
     const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     Tensor p[2] = {weight_ ? *weight_ : Tensor(), bias_ ? *bias_ : Tensor()};
     for (int k = 0; k < 2; ++k) {

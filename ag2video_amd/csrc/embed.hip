@@ -697,7 +697,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
 
 // ---------------------------------------------------------------- host
 static bool embed_ok(int dtype, int idx_bytes, long long n, long long V, int D) {
-    return dtype >= AG2V_F32 && dtype <= AG2V_F16 && (idx_bytes == 4 || idx_bytes == 8) && n > 0 && n < (1LL << 31) && V > 0 && V < (1LL << 31) - 1 && D > 0;
+    return dtype >= AG2V_F32 && dtype <= AG2V_F16 && (idx_bytes == 4 || idx_bytes == 8) && n > 0 && n < (1LL << 31) && V > 0 && V < (1LL << 31) - 1 && D > 0 && D < (1 << 30);
 }
 static int log2_up(long long v) {
     int l = 0;

@@ -2341,7 +2341,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act='silu', slop
     channels are adjacent are read in place (a channel slice; ``t.permute(0, 2, 3, 1)`` of a channels-last NCHW tensor).  Gradients for x,
     weight and bias; h and the activation's derivative are computed again from x, so the tape holds x and two numbers per group.  Sums in
     fp32 in a fixed order (no atomics); y and dx of a sample do not depend on the rest of the batch.  No second
-    derivative (a backward pass with create_graph=True is refused).  Fewer than 2^24 (sample, group) pairs."""
+    derivative (a backward pass with create_graph=True is refused).  Fewer than 2^24 (sample, group) pairs,
+    2^30 positions and channels."""
     return _lib.elem_ops().group_norm_act(x, groups, weight, bias, eps, act, slope)
 
 

@@ -376,8 +376,8 @@ int ag2v_embedding_bwd(const long long* idx, const float* dout, float* dtable, i
  * apart, the tokens idx (int32 or int64: idx_bytes 4 / 8) idx_stride elements.  A token outside [0,V) reads nothing and gives a row of NaN.
  * Gradient: dtable[v,:] = scale * (sum of the rows dout[i,:] with idx_i = v), written densely ([V,D], contiguous; rows no token names and the
  * row padding_idx are zero; padding_idx < 0: none).  The tokens are sorted (stably) and the rows summed in ascending order inside ranges
- * that the sizes alone fix: no atomics, equal calls give equal bits.  dout_stride may be 0 (one row for all).  n, V < 2^31.
- * workspace: ag2v_embed_bwd_workspace_floats() floats. */
+ * that the sizes alone fix: no atomics, equal calls give equal bits.  dout_stride may be 0 (one row for all).  n < 2^31, V < 2^31 - 1,
+ * D < 2^30.  workspace: ag2v_embed_bwd_workspace_floats() floats, 16-byte aligned. */
 int ag2v_embed_fwd(int dtype, const void* idx, int idx_bytes, long long idx_stride, const void* table, long long table_stride, void* out,
                    long long n, long long V, int D, float scale, void* stream);
 size_t ag2v_embed_bwd_workspace_floats(int dtype, long long n, long long V, int D);
@@ -388,7 +388,8 @@ int ag2v_embed_bwd(int dtype, const void* idx, int idx_bytes, long long idx_stri
 /* Group norm with an activation, channels last: x[N,S,C] (strides x_sample / x_row in elements, channels adjacent), y contiguous,
  * weight / bias [C] of param_dtype (AG2V_F32 or dtype) or NULL (1 / 0), mean / rstd fp32 [N,groups] written for the backward pass.
  * act: 0 none, 1 silu, 2 leaky relu of `slope`.  Backward: dx (contiguous), dweight, dbias (param_dtype); each may be NULL.
- * No atomics: equal calls give equal bits.  workspace: ag2v_group_norm_workspace_floats(..., backward) floats. */
+ * No atomics: equal calls give equal bits, and a sample's y and dx do not depend on the batch.  N * groups < 2^24; S, C < 2^30.
+ * workspace: ag2v_group_norm_workspace_floats(..., backward) floats, 16-byte aligned. */
 size_t ag2v_group_norm_workspace_floats(int dtype, int N, int S, int C, int groups, int backward);
 int ag2v_group_norm_fwd(int dtype, const void* x, long long x_sample, long long x_row, const void* weight, const void* bias, int param_dtype,
                         void* y, float* mean, float* rstd, int N, int S, int C, int groups, float eps, int act, float slope,

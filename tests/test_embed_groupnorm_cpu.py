@@ -28,7 +28,7 @@ def test_embed_entry_points_refuse():
     lib, p = _entry()
     fwd = dict(dtype=0, idx=p, ib=8, istride=1, table=p, tstride=8, out=p, n=4, V=5, D=8, scale=1.0, stream=None)
     for change in (dict(dtype=3), dict(dtype=-1), dict(idx=None), dict(table=None), dict(out=None), dict(ib=2), dict(n=0), dict(n=-1), dict(n=1 << 31),
-                   dict(V=0), dict(V=1 << 31), dict(D=0), dict(tstride=7)):
+                   dict(V=0), dict(V=1 << 31), dict(D=0), dict(D=1 << 30), dict(tstride=7)):
         assert lib.ag2v_embed_fwd(*{**fwd, **change}.values()) == -1, change
     need = lib.ag2v_embed_bwd_workspace_floats(0, 5000, 5, 8)
     bwd = dict(dtype=0, idx=p, ib=8, istride=1, dout=p, dstride=8, dtable=p, n=5000, V=5, D=8, scale=1.0, pad=-1, ws=p, nws=need, stream=None)
@@ -37,16 +37,17 @@ def test_embed_entry_points_refuse():
     for n, V, D in ((100000, 50000, 8), (9000, 9000, 700)):
         need = lib.ag2v_embed_bwd_workspace_floats(1, n, V, D)
         big = {**bwd, 'dtype': 1, 'n': n, 'V': V, 'D': D}
-        if need:
-            assert lib.ag2v_embed_bwd(*{**big, 'nws': need - 1}.values()) == -1
-            assert lib.ag2v_embed_bwd(*{**big, 'ws': None, 'nws': need}.values()) == -1
+        assert need > 0
+        assert lib.ag2v_embed_bwd(*{**big, 'nws': need - 1}.values()) == -1
+        assert lib.ag2v_embed_bwd(*{**big, 'ws': None, 'nws': need}.values()) == -1
+        assert lib.ag2v_embed_bwd(*{**big, 'ws': ctypes.c_void_p(4100), 'nws': need}.values()) == -1
     assert lib.ag2v_embed_bwd_workspace_floats(0, 0, 5, 8) == 0 and lib.ag2v_embed_bwd_workspace_floats(9, 10, 5, 8) == 0
 
 
 def test_group_norm_entry_points_refuse():
     lib, p = _entry()
     fwd = dict(dtype=0, x=p, xs=24, xr=8, w=p, b=p, pt=0, y=p, mean=p, rstd=p, N=2, S=3, C=8, G=2, eps=1e-5, act=1, slope=0.2, ws=p, nws=1 << 20, stream=None)
-    for change in (dict(dtype=3), dict(pt=5), dict(x=None), dict(y=None), dict(mean=None), dict(rstd=None), dict(N=0), dict(S=0), dict(S=-4), dict(C=0),
+    for change in (dict(dtype=3), dict(pt=5), dict(x=None), dict(y=None), dict(mean=None), dict(rstd=None), dict(N=0), dict(S=0), dict(S=-4), dict(S=1 << 30), dict(C=0), dict(N=1 << 23), dict(pt=1),
                    dict(G=0), dict(G=3), dict(eps=-1.0), dict(eps=float('nan')), dict(act=3), dict(act=-1)):
         assert lib.ag2v_group_norm_fwd(*{**fwd, **change}.values()) == -1, change
     bwd = dict(dtype=0, dy=p, ds=24, dr=8, x=p, xs=24, xr=8, w=p, b=p, pt=0, mean=p, rstd=p, dx=p, dw=p, db=p, N=2, S=3, C=8, G=2, act=1, slope=0.2,
@@ -56,9 +57,10 @@ def test_group_norm_entry_points_refuse():
     for backward, entry, base in ((0, lib.ag2v_group_norm_fwd, fwd), (1, lib.ag2v_group_norm_bwd, bwd)):
         big = {**base, 'N': 4, 'S': 100000, 'C': 64, 'G': 4}
         need = lib.ag2v_group_norm_workspace_floats(0, 4, 100000, 64, 4, backward)
-        if need:
-            assert entry(*{**big, 'nws': need - 1}.values()) == -1
-            assert entry(*{**big, 'ws': None, 'nws': need}.values()) == -1
+        assert need > 0
+        assert entry(*{**big, 'nws': need - 1}.values()) == -1
+        assert entry(*{**big, 'ws': None, 'nws': need}.values()) == -1
+        assert entry(*{**big, 'ws': ctypes.c_void_p(4100), 'nws': need}.values()) == -1
 
 
 def test_reference_gradients_against_differences():
