@@ -16,6 +16,7 @@
 // After a sort of all tokens, embed_sum_kernel walks equal shares of the sorted order -- a long run of one token costs no more than many short ones --
 // and writes every row whose tokens lie inside one workgroup's share; embed_join_kernel adds the rest up, in order.  No atomics on
 // floating-point values: equal calls give equal bits.
+// Figures below: one MI355X, medians of a kernel trace; a 1 GiB copy reads and writes 5.1 TB/s there.
 #include "elem.h"
 
 __device__ __forceinline__ long long token_at(const void* idx, int wide, long long stride, long long i) {
@@ -61,7 +62,8 @@ __device__ __forceinline__ void join_groups(float (&acc)[V], float* sh, int lsh)
 
 // ---------------------------------------------------------------- lookup
 // 2^lsh lanes a row, 16 bytes a lane, four rows in flight a thread.  The last vector of a row whose width is no multiple of the vector
-// moves back to end with the row (store_row).
+// moves back to end with the row (store_row).  134 MB of 27 words' rows (bf16, 128 wide) in 23 us, 5.8 TB/s written: memory.  102 MB of 50001 words'
+// (fp16, 389 wide) in 27 us: the rows' reads, which the caches serve in part, come on top.  Ten rows in 2.0 us: the launch.
 template <class E, bool NT>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__ idx, int wide, long long istride,
                                                         const typename E::T* __restrict__ table, long long tstride,
@@ -97,6 +99,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__
 }
 
 // ---------------------------------------------------------------- gradient: one launch for few rows and few tokens
+// 1280 tokens of 24 words, 128 fp32: 5.0 us, bound by the chain tokens - list - rows - join.
 #define PICK_MAX 2048
 #define PICK_THREADS 1024
 template <class E>
@@ -190,7 +193,8 @@ __device__ __forceinline__ void store_part(float* p, int D, const float (&v)[V])
 // ---------------------------------------------------------------- gradient: tiles of tokens, for few rows
 // A workgroup sorts T tokens by counting (ranks within a wave by matching the keys' bits over ballots, then over waves), its groups of lanes
 // walk equal shares of the sorted tile as in embed_sum_kernel below, and the sum of each token that occurs goes to part[tile][token][:],
-// count[tile][token] says how often it does.  No pass over the tokens but this one.
+// count[tile][token] says how often it does.  No pass over the tokens but this one.  131072 tokens of 27 words, 128 fp32 (67 MB): 22.6 us, 3.0 TB/s,
+// and 4.1 us for the join; 2 workgroups of 16 groups a CU have eight rows a group in flight, and the sort (some 4 us) is not hidden.
 #define TILE_THREADS 512
 #define TILE_MIN 512
 #define TILE_MAX 2048
@@ -201,7 +205,7 @@ struct TileArgs {
     int* count;
     float* part;
     long long istride, dstride;
-    int wide, n, V, D, pad, lsh, T, bits, tiles;
+    int wide, n, V, D, pad, lsh, jlsh, T, bits, tiles;
     float scale;
 };
 template <class E, bool NT>
@@ -331,14 +335,14 @@ __global__ __launch_bounds__(TILE_THREADS) void embed_tile_kernel(TileArgs a) {
     }
 }
 
-// dtable[v] = scale * the tiles' sums of token v, in order: 2^lsh lanes a column share, the tiles shared over the groups.
-template <class E>
-__global__ __launch_bounds__(PICK_THREADS) void embed_tile_join_kernel(TileArgs a) {
+// dtable[v] = scale * the tiles' sums of token v, in order: 2^jlsh lanes a row, the tiles shared over the groups of lanes.
+template <class E, int THREADS>
+__global__ __launch_bounds__(THREADS) void embed_tile_join_kernel(TileArgs a) {
     constexpr int U = 8;
-    __shared__ float sh[PICK_THREADS * E::V];
+    __shared__ float sh[THREADS * E::V];
     const int v = blockIdx.x % a.V, slice = blockIdx.x / a.V;
-    const int lane = threadIdx.x & ((1 << a.lsh) - 1), grp = threadIdx.x >> a.lsh, ng = PICK_THREADS >> a.lsh;
-    const int c0 = ((slice << a.lsh) + lane) * E::V, c = a.D < E::V ? 0 : min(c0, a.D - E::V);
+    const int lane = threadIdx.x & ((1 << a.jlsh) - 1), grp = threadIdx.x >> a.jlsh, ng = THREADS >> a.jlsh;
+    const int c0 = ((slice << a.jlsh) + lane) * E::V, c = a.D < E::V ? 0 : min(c0, a.D - E::V);
     const int share = (a.tiles + ng - 1) / ng, q1 = min(a.tiles, (grp + 1) * share);
     float acc[E::V] = {};
     if (c0 < a.D)
@@ -357,7 +361,7 @@ __global__ __launch_bounds__(PICK_THREADS) void embed_tile_join_kernel(TileArgs 
                     for (int k = 0; k < E::V; ++k) acc[k] += x[u][k];
                 }
         }
-    join_groups<E::V, PICK_THREADS>(acc, sh, a.lsh);
+    join_groups<E::V, THREADS>(acc, sh, a.jlsh);
     if (grp == 0 && c0 < a.D) {
 #pragma unroll
         for (int k = 0; k < E::V; ++k) acc[k] *= a.scale;
@@ -381,7 +385,8 @@ __device__ __forceinline__ void clear_share(char* p, long long bytes, int blk, i
 // Workgroup b ranks tokens [i0, i0 + 32), i0 = 32 b: rank_i = #{j : k_j < k_i} + #{j < i : k_j = k_i}.  All keys go to LDS; a lane holds k_i
 // (lanes t and t + 32 the same one) and walks its share of j, four broadcast keys a read, a compare and an add with carry each: 2 n^2 / 64
 // vector instructions over the whole chip.  Before i0 equal keys count (k_j < k_i + 1), behind the 32 they do not; the 32 themselves are
-// compared with their positions.  Workgroups beyond the ranking ones clear the table's gradient.
+// compared with their positions.  Workgroups beyond the ranking ones clear the table's gradient.  8192 tokens and a table of 64 MB: 18 us, of
+// which the clearing alone is 10 to 12.
 #define RANK_MAX 8192
 #define RANK_T 32
 #define RANK_THREADS 1024
@@ -433,6 +438,8 @@ __global__ __launch_bounds__(RANK_THREADS) void embed_rank_kernel(const void* __
 // A pass sorts by `bits` <= 9 bits of the key, stably.  Each workgroup owns `rounds` * 2048 consecutive entries.  hist: how often each digit
 // occurs in each workgroup's share, counts[workgroup][digit].  scatter: a workgroup reads all counts, which gives where its entries of
 // each digit begin, ranks its entries (within a wave by matching digits over ballots, then over waves, then over rounds) and writes them.
+// 131071 tokens: hist 4.2 us (8.4 with a table of 39 MB to clear), scatter 10.9: the chain counts - scan - ranks - stores, twice for
+// 50001 words.  Tiles of 1024 tokens or 4096 were slower (12 and 13 us a scatter).
 #define RADIX_BITS 9
 #define RADIX_N (1 << RADIX_BITS)
 #define RADIX_THREADS 512
@@ -549,6 +556,7 @@ __global__ __launch_bounds__(RADIX_THREADS) void embed_scatter_kernel(RadixSrc s
 // share goes to the table at once.  The end of one that began earlier goes to LDS (head), and the group where a segment begins and goes on
 // adds the heads behind its own part.  flags: 1 the share begins inside a segment, 2 which fills it and goes on, 4 a segment begins in the
 // share and goes on.  What began before the workgroup or goes on behind it goes to part[0 / 1][workgroup][:] for embed_join_kernel.
+// 102 MB of rows (131071 x 389 fp16, in the order of 50001 words) in 33 us and 21 MB written, 3.7 TB/s: rows of 778 bytes in no order.
 struct SumArgs {
     const int *skey, *order;
     const void* dout;
@@ -650,7 +658,8 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
     }
 }
 
-// The segments that cross workgroups of embed_sum_kernel: the workgroup where one begins adds its tail and the heads behind it.
+// The segments that cross workgroups of embed_sum_kernel: the workgroup where one begins adds its tail and the heads behind it.  8.6 us where the
+// longest has 8400 tokens, 5 us else: five loads that wait for each other.
 template <class E>
 __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
     __shared__ float sh[256 * E::V];
@@ -710,6 +719,7 @@ static int vec_of(int dtype) { return dtype == AG2V_F32 ? ElemF32::V : ElemBF16:
 struct EmbedPlan {
     bool pick, tile, rank;
     int lsh, slices, L, nblk;       // sums
+    int jlsh, jslices;              // join of tiles
     int T, tiles, bits, passes, rounds, nb;   // tiles; radix
     long long npad, words;          // workspace: sorted keys and positions, their ping-pong, counts, parts
 };
@@ -719,7 +729,9 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
     p.lsh = log2_up(cv < 64 ? cv : 64);
     if (p.lsh < 3) p.lsh = 3;       // at most 32 groups a workgroup
     p.slices = (int)((cv + (1 << p.lsh) - 1) >> p.lsh);
-    // one workgroup may get all n tokens: at most 64 rows a group of lanes then
+    // One workgroup may get all n tokens: at most 64 rows a group of lanes then (2156 equal tokens of 136 fp16 took 64 us in groups of 8 times as
+    // many rows, 18 us by ranks).  Every row costs a workgroup: 2000 tokens of 64 fp32, lookup and gradient, take 12.4 us with 1024 rows (by
+    // ranks 16.9) and 18.9 with 2048 (17.1).
     p.pick = n <= 64LL * (PICK_THREADS >> p.lsh) && n <= PICK_MAX && V * p.slices <= 1024;
     if (p.pick) return p;
     // about 256 tiles, at most 512, whose sums (fp32, V rows a tile) are at most a quarter of the bytes of the rows summed: 131072 tokens of 27
@@ -728,6 +740,8 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
     while (p.T < TILE_MAX && n >= 512LL * p.T) p.T *= 2;
     p.tile = V * 16 <= (dtype == AG2V_F32 ? 4 : 2) * p.T && n <= 512LL * TILE_MAX;
     if (p.tile) {
+        p.jlsh = p.lsh;
+        p.jslices = p.slices;
         if (p.lsh > 4) {                // 16 lanes a row: shares of 16 tokens at least, and more workgroups
             p.lsh = 4;
             p.slices = (int)((cv + 15) >> 4);
@@ -740,7 +754,8 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
     // counting takes 6.2 us for 2156 tokens, 10.5 for 5849, 25 for 11925; a radix pass 12: one pass (V < 512) is faster from 6000 tokens on,
     // two or more from about 11000
     p.rank = n <= (V < RADIX_N ? RANK_MAX * 3 / 4 : RANK_MAX);
-    // entries a group walks: enough groups for 4096 waves, 8 .. 64; more only where the workgroups' parts would pass 16384
+    // entries a group walks: enough groups for 4096 waves, 8 .. 64 (for 2048 waves 131072 rows of 389 fp16 take 49 us and not 37; for 8192 the join
+    // of their longest segment 14 us and not 8.6); more only where the workgroups' parts would pass 16384
     const int ng = 256 >> p.lsh;
     long long L = (n * p.slices << p.lsh) / 64 / 4096;
     L = L < 8 ? 8 : L > 64 ? 64 : 1LL << (log2_up(L + 1) - 1);
@@ -789,14 +804,17 @@ static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istr
     }
     if (p.tile) {
         int* count = (int*)workspace;
-        const TileArgs t = {idx, dout, dtable, count, workspace + ((long long)p.tiles * V + 3) / 4 * 4, istride, dstride, wide, n, V, D, pad, p.lsh, p.T, p.bits,
+        const TileArgs t = {idx, dout, dtable, count, workspace + ((long long)p.tiles * V + 3) / 4 * 4, istride, dstride, wide, n, V, D, pad, p.lsh, p.jlsh, p.T, p.bits,
                             p.tiles, scale};
         if ((long long)n * D * (long long)sizeof(typename E::T) > AG2V_NT_LOAD_BYTES)
             hipLaunchKernelGGL((embed_tile_kernel<E, true>), dim3(p.tiles * p.slices), dim3(TILE_THREADS), 0, st, t);
         else
             hipLaunchKernelGGL((embed_tile_kernel<E, false>), dim3(p.tiles * p.slices), dim3(TILE_THREADS), 0, st, t);
         AG2V_CHECK_LAUNCH();
-        hipLaunchKernelGGL(embed_tile_join_kernel<E>, dim3(V * p.slices), dim3(PICK_THREADS), 0, st, t);
+        if (p.tiles > 64)      // few tiles need few groups of lanes, and there may be many rows
+            hipLaunchKernelGGL((embed_tile_join_kernel<E, 1024>), dim3(V * p.jslices), dim3(1024), 0, st, t);
+        else
+            hipLaunchKernelGGL((embed_tile_join_kernel<E, 256>), dim3(V * p.jslices), dim3(256), 0, st, t);
         AG2V_CHECK_LAUNCH();
         return AG2V_OK;
     }

@@ -5,6 +5,11 @@
 //   backward, dz = dy act'(z), A[n,c] = sum_s dz, B[n,c] = sum_s dz h:
 //     db = sum_n A, dw = sum_n B, s1 = sum_{c in g} w A, s2 = sum_{c in g} w B, dx = rstd (w dz - (s1 + h s2) / M)
 // Every sum is in fp32; z and h are computed again in the backward pass from x and the two statistics of a group.
+//
+// Memory bounds all of it: forward x is read and y written, backward x and dy are read and dx written.  A (sample, set of groups) that fits
+// the registers of a workgroup is read once, in one launch (gn_slab_*).  A larger one is read twice: parts of a sample's positions give
+// partial sums (gn_stats, gn_bwd_sums), a join gives the group's, and a second pass over the map writes the result (gn_apply, gn_bwd_dx).
+// Figures below: one MI355X, medians of a kernel trace; a 1 GiB copy reads and writes 5.1 TB/s there, 128 MiB of cached data 8.5 TB/s.
 #include "elem.h"
 
 #define ACT_NONE 0
@@ -126,7 +131,9 @@ static int log2_up(long long v) {
 
 // ---------------------------------------------------------------- one launch: a slab's values stay in registers
 // T threads own all S positions of kg adjacent groups of one sample, U vectors a thread, read once: mean, then the squared deviations from
-// it, then the result.  blockDim / T slabs a workgroup.  ONE: a thread's vector touches one group (Cg a multiple of the vector, or kg = 1);
+// it, then the result.  blockDim / T slabs a workgroup.  Small maps: 6.0 us for 1 x 64 x 1024 bf16 and for 8 x 64 x 1024 fp32, of which an empty
+// kernel's launch is 2 and the chain load - sum - squares - store the rest.  20.4 us for 8 x 4096 x 256 fp16 in 32 groups, whose rows are
+// one vector each: 1.6 TB/s, bound by 16-byte pieces of cache lines.  ONE: a thread's vector touches one group (Cg a multiple of the vector, or kg = 1);
 // otherwise sums and statistics are per channel.
 struct GnSlab {
     int T, kg, nsets, lc, rows, slots, wg, llg;   // threads, groups, sets of groups a sample, log2 of vectors a row, rows at a time, LDS slots and columns a group, log2 of lanes a group
@@ -242,7 +249,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
     }
 }
 
-// Backward on slabs: x and dy of a slab in registers.  A workgroup keeps its set of groups and walks samples, `walkers` apart, so that the
+// Backward on slabs: x and dy of a slab in registers (7.3 us for 8 x 64 x 1024 fp32, bound by the chain of loads and joins).  A workgroup keeps its set of groups and walks samples, `walkers` apart, so that the
 // parameters' gradients leave it once: ab[walker][C] = (sum dz, sum dz h) over its samples.  Without ONE the statistics are per channel and
 // take 512 threads of 256 registers.
 template <class E, int ACT, int U, bool ONE>
@@ -417,6 +424,7 @@ __device__ __forceinline__ GnWhere where_of(const GnArgs& a, const GnParts& p, i
 // sum of squares about it is at most (count + 1) times the one about the thread's mean, and nothing cancels that matters, whatever the mean.
 // Threads, waves and channels then join pairwise as (count, mean, squares about the mean).
 // part[n][g][q * tg + (tile - the group's first tile)] = (count, mean, squares, 0)
+// 134 MB (16 x 65536 x 64 bf16) in 34 us, 4.0 TB/s; the joins at the end of every 32 KB are what keeps it below the copy's rate.
 template <class E>
 __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, float4* part) {
     constexpr int V = E::V, U = 8;
@@ -512,7 +520,8 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, floa
     }
 }
 
-// A wave per (sample, group): the mean of its parts' means, then the squares about it, in fp64.
+// A wave per (sample, group): the mean of its parts' means, then the squares about it, in fp64.  4.7 us for 512 groups of 256 parts, two
+// rounds of loads and shuffles.
 template <int V>
 __global__ __launch_bounds__(256) void gn_stats_join_kernel(GnArgs a, GnParts p, const float4* part) {
     const int id = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
@@ -588,6 +597,8 @@ __device__ __forceinline__ int join_here(const GnArgs& a, const GnParts& p, cons
     return gl;
 }
 
+// y.  `part` where the groups' parts are joined here.  268 MB (16 x 65536 x 64 bf16) in 45 us, 6.0 TB/s: memory, half of it from the Infinity
+// Cache that the statistics have filled.
 template <class E, int ACT, bool NT>
 __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p, const float4* part) {
     constexpr int V = E::V, U = 4;
@@ -629,7 +640,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p, cons
     }
 }
 
-// part[n][q][c] = (sum dz, sum dz h) over the part's positions
+// part[n][q][c] = (sum dz, sum dz h) over the part's positions.  268 MB (4 x 65536 x 256 bf16) in 51 us, 5.3 TB/s: memory.
 template <class E, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, float2* part) {
     constexpr int V = E::V, U = 4;
@@ -691,7 +702,8 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
     }
 }
 
-// A workgroup per (sample, group): the parts of its channels, in order; ab[n][c], and the group's (s1 / M, s2 / M) to coef[n][g].
+// A workgroup per (sample, group): the parts of its channels, in order; ab[n][c], and the group's (s1 / M, s2 / M) to coef[n][g].  5.6 us for
+// 128 groups of 8 channels in 512 parts.
 __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int lcw, const float2* part, float2* ab, float2* coef) {
     __shared__ float2 sh[256];
     const int n = blockIdx.x / a.G, g = blockIdx.x - n * a.G;
@@ -771,7 +783,8 @@ __device__ __forceinline__ void params_of(const GnArgs& a, int blk, int rows, co
 }
 __global__ __launch_bounds__(256) void gn_params_kernel(GnArgs a, int rows, const float2* ab) { params_of(a, blockIdx.x, rows, ab); }
 
-// dx; the first `pblocks` workgroups sum the parameters' gradients instead.  NT: 1 stores past the caches, 2 loads too.
+// dx; the first `pblocks` workgroups sum the parameters' gradients instead.  NT: 1 stores past the caches, 2 loads too.  403 MB (4 x 65536 x 256
+// bf16) in 66 us, 6.1 TB/s: memory.
 template <class E, int ACT, int NT>
 __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef, int pblocks, const float2* ab) {
     constexpr int V = E::V, U = 4;
@@ -835,14 +848,22 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     const int Cg = C / G;
     const auto lcols = [&](int k) { return log2_up(((long long)k * Cg + V - 1) / V); };
     const long long most = backward ? GN_SLAB_BWD : GN_SLAB_FWD;        // vectors a slab
-    // groups of a slab: rows of 128 bytes where that fits, so that slabs share no cache line
+    // Groups of a slab: rows of 64 bytes, so that few slabs share a cache line.  Where what the slabs of a sample read is small enough to stay in an
+    // XCD's L2, that does not matter and more workgroups do: 512 vectors are enough then (4 x 1000 x 320 fp16 in 40 groups, forward: one group a slab
+    // 7.5 us, four 9.6, eight 13.2; 16 x 100 x 256 fp32 in 64 groups: 6.5, 5.8 and 6.0), or one group of an odd width (2 x 120 x 90 bf16 in 6 groups,
+    // training: 16.5 us, two groups 20.2).
+    const long long bytes = (long long)S * C * (16 / V) * (backward ? 2 : 1);
+    const bool small = bytes <= (1 << 20);
     int kg = 1;
-    while (kg < G && (long long)kg * Cg < 8 * V && lcols(kg + 1) <= 3 && ((long long)S << lcols(kg + 1)) <= most) ++kg;
+    while (kg < G && (long long)kg * Cg < 4 * V && lcols(kg + 1) <= 2 && ((long long)S << lcols(kg + 1)) <= most &&
+           !(small && (((long long)S << lcols(kg)) >= 512 || (Cg % V && 4 * Cg >= V)) && (S <= 2048 || (long long)kg * Cg >= V)))
+        ++kg;
     const int lc = lcols(kg);
-    // narrow rows: every cache line would be read by many slabs, in pieces (13 x 1085 x 1560 fp16 in 195 groups, one vector a row: 147 us a
-    // training pass, 72 us in parts; 11 x 4181 x 45 fp32 in 15 groups, 12 bytes a row: 49 and 37 us).  Forward, rows of whole vectors are no
-    // slower here (8 x 4096 x 256 fp16 in 32 groups: 20.8 us, in parts 22) and take one launch.
-    if (kg < G && (backward ? (long long)kg * Cg < 4 * V : (long long)kg * Cg < 2 * V && Cg % V)) return false;
+    // Narrow rows of a larger map: every cache line would be fetched by many slabs, in pieces (13 x 1085 x 1560 fp16 in 195 groups, one vector a
+    // row: 147 us a training pass, 72 us in parts; 11 x 4181 x 45 fp32 in 15 groups, 12 bytes a row: 49 and 37 us).  Forward, rows of whole
+    // vectors are no slower here (8 x 4096 x 256 fp16 in 32 groups: 20.4 us, in parts 22) and take one launch.
+    if (kg < G && (long long)kg * Cg < V && S > 2048) return false;
+    if (!small && kg < G && (backward ? (long long)kg * Cg < 4 * V : (long long)kg * Cg < 2 * V && Cg % V)) return false;
     if (lc > 10 || ((long long)S << lc) > most) return false;
     const bool one = kg == 1 || Cg % V == 0;
     const int maxT = backward && !one ? 512 : 1024, maxU = backward ? 2 : one ? 8 : 4;
