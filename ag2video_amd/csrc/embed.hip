@@ -194,11 +194,14 @@ __device__ __forceinline__ void store_part(float* p, int D, const float (&v)[V])
 // A workgroup sorts T tokens by counting (ranks within a wave by matching the keys' bits over ballots, then over waves), its groups of lanes
 // walk equal shares of the sorted tile as in embed_sum_kernel below, and the sum of each token that occurs goes to part[tile][token][:],
 // count[tile][token] says how often it does.  No pass over the tokens but this one.  131072 tokens of 27 words, 128 fp32 (67 MB): 22.6 us, 3.0 TB/s,
-// and 4.1 us for the join; 2 workgroups of 16 groups a CU have eight rows a group in flight, and the sort (some 4 us) is not hidden.
+// and 4.1 us for the join; 2 workgroups of 32 groups a CU have eight rows a group in flight, and the sort (some 4 us) is not hidden.
 #define TILE_THREADS 512
 #define TILE_MIN 512
 #define TILE_MAX 2048
 #define TILE_BITS 9
+// More tiles than this are joined by 1024 threads in groups of 16 lanes, fewer by 256 in groups of up to 64: 5 tiles of 89 rows, 1400 wide, took
+// 27 us a training pass so and 40 the other way; 256 tiles of 27 rows, 128 wide, 4.1 us a join and 5.4 in wider groups.
+#define TILE_JOIN_WIDE 64
 struct TileArgs {
     const void *idx, *dout;
     void* dtable;
@@ -747,6 +750,10 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
             p.slices = (int)((cv + 15) >> 4);
         }
         p.tiles = (int)((n + p.T - 1) / p.T);
+        if (p.tiles > TILE_JOIN_WIDE) {
+            p.jlsh = p.lsh;
+            p.jslices = p.slices;
+        }
         p.bits = log2_up(V + 1);
         p.words = ((long long)p.tiles * V + 3) / 4 * 4 + (long long)p.tiles * V * D;
         return p;
@@ -811,7 +818,7 @@ static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istr
         else
             hipLaunchKernelGGL((embed_tile_kernel<E, false>), dim3(p.tiles * p.slices), dim3(TILE_THREADS), 0, st, t);
         AG2V_CHECK_LAUNCH();
-        if (p.tiles > 64)      // few tiles need few groups of lanes, and there may be many rows
+        if (p.tiles > TILE_JOIN_WIDE)
             hipLaunchKernelGGL((embed_tile_join_kernel<E, 1024>), dim3(V * p.jslices), dim3(1024), 0, st, t);
         else
             hipLaunchKernelGGL((embed_tile_join_kernel<E, 256>), dim3(V * p.jslices), dim3(256), 0, st, t);

@@ -478,9 +478,9 @@ def test_run_together(shape, device):
     R.check('dtable', dt, total, off * (1 + R.U) + 4 * R.U * total.abs())
 
 
-def test_other_stream_and_replay(device):
+@pytest.mark.parametrize("V,D,shape", [(20, 16, (2, 30)), (300, 48, (4, 900)), (20, 48, (2, 9000)), (70000, 20, (3, 7000))], ids=str)
+def test_other_stream_and_replay(V, D, shape, device):
     """Forward and backward on a side stream, then captured into a graph and replayed on new values between eager calls: the same bits."""
-    V, D, shape = 300, 48, (4, 900)
     torch.manual_seed(0)
     idx = torch.randint(V, shape, device=device)
     fresh = [torch.randn(V, D, device=device), torch.randn(D, device=device), torch.randn(D, device=device)]
@@ -548,6 +548,55 @@ def test_calls_on_two_streams_at_once(device):
                 got.append((k % 2, (embed, norm)[k % 2]()))
     torch.cuda.synchronize()
     assert all(torch.equal(t, want[k]) for k, t in got)
+
+
+def test_calls_of_two_threads(device):
+    """Each thread on a stream of its own, forward and backward."""
+    import threading
+    from ag2video_amd import ops
+    x, dy = torch.randn(3, 700, 64, device=device), torch.randn(3, 700, 64, device=device)
+    idx, table, dout = torch.randint(900, (9000,), device=device), torch.randn(900, 24, device=device), torch.randn(9000, 24, device=device)
+
+    def norm():
+        t = x.detach().requires_grad_(True)
+        return torch.autograd.grad(ops.group_norm_act(t, 8), t, dy)[0]
+
+    def embed():
+        t = table.detach().requires_grad_(True)
+        return torch.autograd.grad(ops.embedding_scaled(idx, t, 0.5), t, dout)[0]
+
+    want, got = (norm(), embed()), []
+    torch.cuda.synchronize()
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            mine = [(norm, embed)[k]() for _ in range(20)]
+            stream.synchronize()
+        got.extend((k, t) for t in mine)
+
+    threads = [threading.Thread(target=work, args=(k % 2,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 80 and all(torch.equal(t, want[k]) for k, t in got)
+
+
+def test_parameters_inside_flat_buffers(device):
+    """Tables and norm parameters that are views of a flat buffer at any element offset (as the fused optimizer keeps them)."""
+    from ag2video_amd import ops
+    flat = _randn(2000, seed=1).to(device)
+    for off in (1, 2, 3, 5):
+        w, b, table = flat[off:off + 52], flat[100 + off:152 + off], flat[200 + off:200 + off + 19 * 52].view(19, 52)
+        idx = _tokens(300, 19, off)
+        ref = R.embedding(idx, table.cpu(), 2.0, None)
+        rows = ops.embedding_scaled(idx.to(device), table, 2.0)
+        R.check('rows', rows, *ref)
+        x = rows.view(3, 100, 52)
+        for S in (100, 50):
+            want = R.group_norm(x[:, :S].cpu(), 13, w.cpu(), b.cpu(), 1e-5, 'silu', 0.2)
+            R.check('y', ops.group_norm_act(x[:, :S], 13, w, b), *want['y'])
 
 
 def test_modules(device):
