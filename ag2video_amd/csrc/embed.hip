@@ -467,7 +467,8 @@ __global__ __launch_bounds__(RADIX_THREADS) void embed_hist_kernel(RadixSrc s, i
     __syncthreads();
     const int mask = (1 << bits) - 1;
     const long long lo = (long long)blockIdx.x * rounds * RADIX_TILE, hi = min((long long)n, lo + (long long)rounds * RADIX_TILE);
-    for (long long e = lo + threadIdx.x; e < hi; e += RADIX_THREADS) atomicAdd(&h[(radix_key(s, (int)e) >> shift) & mask], 1);   // whole numbers: any order, one result
+    for (long long e = lo + threadIdx.x; e < hi; e += RADIX_THREADS)
+        atomicAdd(&h[(radix_key(s, (int)e) >> shift) & mask], 1);          // whole numbers: any order, one result
     __syncthreads();
     counts[blockIdx.x * RADIX_N + threadIdx.x] = h[threadIdx.x];
 }
@@ -709,7 +710,8 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
 
 // ---------------------------------------------------------------- host
 static bool embed_ok(int dtype, int idx_bytes, long long n, long long V, int D) {
-    return dtype >= AG2V_F32 && dtype <= AG2V_F16 && (idx_bytes == 4 || idx_bytes == 8) && n > 0 && n < (1LL << 31) && V > 0 && V < (1LL << 31) - 1 && D > 0 && D < (1 << 30);
+    return dtype >= AG2V_F32 && dtype <= AG2V_F16 && (idx_bytes == 4 || idx_bytes == 8) && n > 0 && n < (1LL << 31) &&
+           V > 0 && V < (1LL << 31) - 1 && D > 0 && D < (1 << 30);
 }
 static int log2_up(long long v) {
     int l = 0;
@@ -738,10 +740,11 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
     p.pick = n <= 64LL * (PICK_THREADS >> p.lsh) && n <= PICK_MAX && V * p.slices <= 1024;
     if (p.pick) return p;
     // about 256 tiles, at most 512, whose sums (fp32, V rows a tile) are at most a quarter of the bytes of the rows summed: 131072 tokens of 27
-    // words, 128 wide, take 23 us so and 33 us by a radix pass; 524288 of 256 words in fp16, half the rows' bytes, 72 and 55 us
+    // words, 128 wide, take 23 us so and 33 us by a radix pass; 524288 of 256 words in fp16, half the rows' bytes, 72 and 55 us.  The keys 0 .. V
+    // have a counter each in LDS
     p.T = TILE_MIN;
     while (p.T < TILE_MAX && n >= 512LL * p.T) p.T *= 2;
-    p.tile = V * 16 <= (dtype == AG2V_F32 ? 4 : 2) * p.T && n <= 512LL * TILE_MAX;
+    p.tile = V * 16 <= (dtype == AG2V_F32 ? 4 : 2) * p.T && V < 1 << TILE_BITS && n <= 512LL * TILE_MAX;
     if (p.tile) {
         p.jlsh = p.lsh;
         p.jslices = p.slices;
@@ -811,8 +814,8 @@ static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istr
     }
     if (p.tile) {
         int* count = (int*)workspace;
-        const TileArgs t = {idx, dout, dtable, count, workspace + ((long long)p.tiles * V + 3) / 4 * 4, istride, dstride, wide, n, V, D, pad, p.lsh, p.jlsh, p.T, p.bits,
-                            p.tiles, scale};
+        const TileArgs t = {idx, dout, dtable, count, workspace + ((long long)p.tiles * V + 3) / 4 * 4, istride, dstride, wide, n, V, D, pad,
+                            p.lsh, p.jlsh, p.T, p.bits, p.tiles, scale};
         if ((long long)n * D * (long long)sizeof(typename E::T) > AG2V_NT_LOAD_BYTES)
             hipLaunchKernelGGL((embed_tile_kernel<E, true>), dim3(p.tiles * p.slices), dim3(TILE_THREADS), 0, st, t);
         else
@@ -832,8 +835,8 @@ static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istr
     SumArgs a = {skey, order, dout, dtable, (float*)(order + p.npad), dstride, n, V, D, p.lsh, p.L, p.nblk, scale};
     if (p.rank) {
         const int rank_blocks = ceil_div(n, RANK_T);
-        hipLaunchKernelGGL(embed_rank_kernel, dim3(rank_blocks + clearers), dim3(RANK_THREADS), 0, st, idx, wide, istride, skey, order, n, V, pad, rank_blocks,
-                           (char*)dtable, bytes);
+        hipLaunchKernelGGL(embed_rank_kernel, dim3(rank_blocks + clearers), dim3(RANK_THREADS), 0, st, idx, wide, istride, skey, order, n, V,
+                           pad, rank_blocks, (char*)dtable, bytes);
         AG2V_CHECK_LAUNCH();
     } else {
         int* counts = (int*)(a.part + 2LL * p.nblk * D);

@@ -27,7 +27,8 @@ class Embedding(nn.Embedding):
     def forward(self, idx):
         if self.scale is None and self.padding_idx is None and self.weight.dtype == torch.float32:
             return ops.embedding(idx, self.weight)
-        return ops.embedding_scaled(idx, self.weight, 1.0 if self.scale is None else self.scale, self.padding_idx)
+        tokens = idx if idx.dtype in (torch.int32, torch.int64) else idx.to(torch.int64)       # (as ops.embedding takes them)
+        return ops.embedding_scaled(tokens, self.weight, 1.0 if self.scale is None else self.scale, self.padding_idx)
 
 
 class GroupNormAct(nn.GroupNorm):

@@ -74,6 +74,16 @@ def test_embedding_scaled_switching_sizes(n, V, D, kind, device):
         _embed_case(device, idx, _randn(V, D, seed=1, dtype=dtype), 1.0, V // 3, _randn(n, D, seed=2, scale=0.1, dtype=dtype), 'embed')
 
 
+@pytest.mark.parametrize("V", [255, 256, 257, 511, 512, 513], ids=str)
+def test_embedding_scaled_large_tiles(V, device):
+    """As many words as a tile of tokens has counters for, and one more; the last tile ends inside, and some tokens take no part."""
+    n = 524288 + 77
+    idx = _tokens(n, V, V, 'skewed')
+    idx[::5] = V
+    for dtype in (torch.float32, torch.float16):
+        _embed_case(device, idx, _randn(V, 4, seed=1, dtype=dtype), 0.5, 3, _randn(n, 4, seed=2, scale=0.05, dtype=dtype), 'embed')
+
+
 def test_embedding_scaled_past_the_caches(device):
     """Results and gradients large enough to go past the caches.  Whole numbers: every product and sum is exact."""
     from ag2video_amd import ops
@@ -616,6 +626,15 @@ def test_modules(device):
     assert torch.equal(plain(idx), ops.embedding(idx, plain.weight))
     half = Embedding(11, 24).to(device).to(torch.bfloat16)
     assert half(idx).dtype == torch.bfloat16
+
+
+def test_module_takes_tokens_of_any_integer_type(device):
+    """A padding_idx changes the operator behind layers.Embedding, not the tokens it takes."""
+    from ag2video_amd.models.layers import Embedding
+    idx = _tokens(40, 11, 1).to(device)
+    emb = Embedding(11, 24, padding_idx=3).to(device)
+    for itype in (torch.uint8, torch.int16, torch.int32):
+        assert torch.equal(emb(idx.to(itype)), emb.weight[idx])
 
 
 def test_no_second_derivative(device):
