@@ -180,8 +180,8 @@ std::pair<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& weight, co
 }
 
 struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, int64_t groups,
-                          double eps, int64_t act, double slope) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_,
+                          int64_t groups, double eps, int64_t act, double slope) {
         const Tensor weight = weight_ ? *weight_ : Tensor(), bias = bias_ ? *bias_ : Tensor();
         auto [y, stats] = norm_forward(x, weight, bias, groups, eps, act, slope);
         ctx->save_for_backward({x, weight, bias, stats});
@@ -245,7 +245,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const std::optional<Tenso
     if (p[0].defined() && p[1].defined())
         TORCH_CHECK(p[0].scalar_type() == p[1].scalar_type(), name, ": weight is ", p[0].scalar_type(), ", bias ", p[1].scalar_type());
     const auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
-    if (at::GradMode::is_enabled() && (wants(x) || wants(p[0]) || wants(p[1]))) 
+    if (at::GradMode::is_enabled() && (wants(x) || wants(p[0]) || wants(p[1])))
         return GroupNormAct::apply(x, given(p[0]), given(p[1]), groups, eps, code, slope);
     return norm_forward(x, p[0], p[1], groups, eps, code, slope).first;
 }

@@ -65,7 +65,8 @@ __device__ __forceinline__ void load_params(const void* p, int ptype, int c, int
 }
 // mean and 1 / std of V channels from c on
 template <int V>
-__device__ __forceinline__ void load_stats(const GnArgs& a, int n, int c, float (&mean)[V], float (&rstd)[V], const float2* coef = nullptr, float2* cf = nullptr) {
+__device__ __forceinline__ void load_stats(const GnArgs& a, int n, int c, float (&mean)[V], float (&rstd)[V], const float2* coef = nullptr,
+                                           float2* cf = nullptr) {
     if (a.Cg % V == 0 && c % V == 0) {
         const int g = n * a.G + c / a.Cg;
         const float m = a.mean[g], r = a.rstd[g];
@@ -131,12 +132,13 @@ static int log2_up(long long v) {
 
 // ---------------------------------------------------------------- one launch: a slab's values stay in registers
 // T threads own all S positions of kg adjacent groups of one sample, U vectors a thread, read once: mean, then the squared deviations from
-// it, then the result.  blockDim / T slabs a workgroup.  Small maps: 6.0 us for 1 x 64 x 1024 bf16 and for 8 x 64 x 1024 fp32, of which an empty
-// kernel's launch is 2 and the chain load - sum - squares - store the rest.  20.4 us for 8 x 4096 x 256 fp16 in 32 groups, whose rows are
-// one vector each: 1.6 TB/s, bound by 16-byte pieces of cache lines.  ONE: a thread's vector touches one group (Cg a multiple of the vector, or kg = 1);
+// it, then the result.  blockDim / T slabs a workgroup.  ONE: a thread's vector touches one group (Cg a multiple of the vector, or kg = 1);
 // otherwise sums and statistics are per channel.
+// 6.0 us for 1 x 64 x 1024 bf16 and for 8 x 64 x 1024 fp32, of which an empty kernel's launch is 2 and the chain load - sum - squares - store
+// the rest.  20 us for 8 x 4096 x 256 fp16 in 32 groups, whose rows are one vector each: 1.6 TB/s, bound by 16-byte pieces of cache lines.
 struct GnSlab {
-    int T, kg, nsets, lc, rows, slots, wg, llg;   // threads, groups, sets of groups a sample, log2 of vectors a row, rows at a time, LDS slots and columns a group, log2 of lanes a group
+    int T, kg, nsets;                  // threads, groups, sets of groups a sample
+    int lc, rows, slots, wg, llg;      // log2 of vectors a row, rows at a time, LDS slots, columns a group there, log2 of lanes a group
     long long nslab;
 };
 
@@ -249,9 +251,9 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
     }
 }
 
-// Backward on slabs: x and dy of a slab in registers (7.3 us for 8 x 64 x 1024 fp32, bound by the chain of loads and joins).  A workgroup keeps its set of groups and walks samples, `walkers` apart, so that the
+// Backward on slabs: x and dy of a slab in registers.  A workgroup keeps its set of groups and walks samples, `walkers` apart, so that the
 // parameters' gradients leave it once: ab[walker][C] = (sum dz, sum dz h) over its samples.  Without ONE the statistics are per channel and
-// take 512 threads of 256 registers.
+// take 512 threads of 256 registers.  7.3 us for 8 x 64 x 1024 fp32, bound by the chain of loads and joins.
 template <class E, int ACT, int U, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a, GnSlab p, int walkers, float2* ab) {
     extern __shared__ float shm[];
