@@ -830,8 +830,11 @@ static int run_bwd(const EmbedPlan& p, const void* idx, int wide, long long istr
     }
     int *skey = (int*)workspace, *order = skey + p.npad;
     const long long bytes = (long long)V * D * (long long)sizeof(typename E::T);
-    const long long cb = (bytes / 16 + 255) / 256;
-    const int clearers = cb < 1 ? 1 : cb < 1024 ? (int)cb : 1024;
+    // one vector a thread: workgroups that walk the table write it slower (4000 tokens of 131072 words, 1024 bf16: 64 us a training pass, 84 with
+    // 1024 workgroups)
+    const int threads = p.rank ? RANK_THREADS : RADIX_THREADS;
+    const long long cb = (bytes / 16 + threads - 1) / threads;
+    const int clearers = cb < 1 ? 1 : cb < 65536 ? (int)cb : 65536;
     SumArgs a = {skey, order, dout, dtable, (float*)(order + p.npad), dstride, n, V, D, p.lsh, p.L, p.nblk, scale};
     if (p.rank) {
         const int rank_blocks = ceil_div(n, RANK_T);
