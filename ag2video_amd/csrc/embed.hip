@@ -388,8 +388,8 @@ __device__ __forceinline__ void clear_share(char* p, long long bytes, int blk, i
 // Workgroup b ranks tokens [i0, i0 + 32), i0 = 32 b: rank_i = #{j : k_j < k_i} + #{j < i : k_j = k_i}.  All keys go to LDS; a lane holds k_i
 // (lanes t and t + 32 the same one) and walks its share of j, four broadcast keys a read, a compare and an add with carry each: 2 n^2 / 64
 // vector instructions over the whole chip.  Before i0 equal keys count (k_j < k_i + 1), behind the 32 they do not; the 32 themselves are
-// compared with their positions.  Workgroups beyond the ranking ones clear the table's gradient.  8192 tokens and a table of 64 MB: 18 us, of
-// which the clearing alone is 10 to 12.
+// compared with their positions.  Workgroups beyond the ranking ones clear the table's gradient.  8192 tokens and a table of 64 MB: 16 us, of
+// which the clearing alone is about 10.
 #define RANK_MAX 8192
 #define RANK_T 32
 #define RANK_THREADS 1024
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(RANK_THREADS) void embed_rank_kernel(const void* __
 // A pass sorts by `bits` <= 9 bits of the key, stably.  Each workgroup owns `rounds` * 2048 consecutive entries.  hist: how often each digit
 // occurs in each workgroup's share, counts[workgroup][digit].  scatter: a workgroup reads all counts, which gives where its entries of
 // each digit begin, ranks its entries (within a wave by matching digits over ballots, then over waves, then over rounds) and writes them.
-// 131071 tokens: hist 4.2 us (8.4 with a table of 39 MB to clear), scatter 10.9: the chain counts - scan - ranks - stores, twice for
+// 131071 tokens: hist 4.0 us (7.5 with a table of 39 MB to clear), scatter 10.9: the chain counts - scan - ranks - stores, twice for
 // 50001 words.  Tiles of 1024 tokens or 4096 were slower (12 and 13 us a scatter).
 #define RADIX_BITS 9
 #define RADIX_N (1 << RADIX_BITS)
