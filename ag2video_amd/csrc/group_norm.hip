@@ -253,7 +253,8 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
 
 // Backward on slabs: x and dy of a slab in registers.  A workgroup keeps its set of groups and walks samples, `walkers` apart, so that the
 // parameters' gradients leave it once: ab[walker][C] = (sum dz, sum dz h) over its samples.  Without ONE the statistics are per channel and
-// take 512 threads of 256 registers.  7.3 us for 8 x 64 x 1024 fp32, bound by the chain of loads and joins.
+// take up to 256 registers a thread; with ONE the bound of 1024 threads keeps them to 128, so that two workgroups of 512 fit a CU (64 x 1024 x 256
+// bf16: 58 us with 128 and 82 with 136).  7.3 us for 8 x 64 x 1024 fp32, bound by the chain of loads and joins.
 template <class E, int ACT, int U, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a, GnSlab p, int walkers, float2* ab) {
     extern __shared__ float shm[];
@@ -518,7 +519,8 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, floa
         }
         for (int o = step >> 1; o > 0; o >>= 1) q += __shfl_xor(q, o, 64);
         if (l == 0)
-            part[((long long)i.n * a.G + g) * p.P * p.tg + i.q * p.tg + i.tile - g * a.Cg / (V << p.lc)] = make_float4(rows * (float)(ch - cl), gm, q, 0.f);
+            part[((long long)i.n * a.G + g) * p.P * p.tg + i.q * p.tg + i.tile - g * a.Cg / (V << p.lc)] =
+                make_float4(rows * (float)(ch - cl), gm, q, 0.f);
     }
 }
 
@@ -842,10 +844,10 @@ struct GnPlan {
     GnParts p;
     long long words, ab, coef;       // workspace in floats; offsets of ab[][C] and coef[N][G] in it
 };
-// Vectors of a slab at most.  Forward, a slab of 4096 takes 20.8 us (8 x 4096 x 256 fp16) and parts 22 us in two launches; backward, x and dy of
-// 4096 vectors took 59 us where the parts take 31.
+// Vectors of a slab at most.  Forward, 8192 (8 x 4096 x 256 fp16: 17 us, in parts 20; 64 x 1961 x 90 fp32 32 and 35).  Backward, where x and dy
+// are held, 1024: the 2000 vectors of 64 x 2000 x 64 fp16 in 8 groups took 55 us a training pass, 44 in parts, and 24 and 19.5 for one sample.
 #define GN_SLAB_FWD 8192
-#define GN_SLAB_BWD 2048
+#define GN_SLAB_BWD 1024
 static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backward) {
     const int Cg = C / G;
     const auto lcols = [&](int k) { return log2_up(((long long)k * Cg + V - 1) / V); };
@@ -865,12 +867,22 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     // row: 147 us a training pass, 72 us in parts; 11 x 4181 x 45 fp32 in 15 groups, 12 bytes a row: 49 and 37 us).  Forward, rows of whole
     // vectors are no slower here (8 x 4096 x 256 fp16 in 32 groups: 20.4 us, in parts 22) and take one launch.
     if (kg < G && (long long)kg * Cg < V && S > 2048) return false;
-    if (!small && kg < G && (backward ? (long long)kg * Cg < 4 * V : (long long)kg * Cg < 2 * V && Cg % V)) return false;
-    if (lc > 10 || ((long long)S << lc) > most) return false;
+    const long long held = (long long)S << lc;
+    if (!small && kg < G && !backward && (long long)kg * Cg < 2 * V && Cg % V) return false;
+    // Backward they are, beyond 512 vectors in rows of up to 32 bytes also on small maps: 64 x 1024 x 256 bf16 in 32 groups took 87 us a training pass, 71 in parts (one sample
+    // 18.8 and 19.1), and 64 x 1000 x 50 fp16 in 10 groups 61 and 46.  Rows of 60 are not: 200 x 90 fp32 in 6 groups 14.3 and 15.6.
+    if (kg < G && backward && ((!small && (long long)kg * Cg < 4 * V) || (held > 512 && (long long)kg * Cg <= 2 * V))) return false;
+    if (lc > 10 || held > most) return false;
     const bool one = kg == 1 || Cg % V == 0;
-    const int maxT = backward && !one ? 512 : 1024, maxU = backward ? 2 : one ? 8 : 4;
+    // 512 threads, which meet sooner and leave room for a second workgroup on the CU: 64 x 256 x 1280 bf16 forward took 50 us with 1024 threads and
+    // takes 31, 64 x 533 x 608 fp16 59 and 37.  1024 for rows that wide, and where the registers of 512 do not hold the slab and at least three
+    // quarters of the lanes work (64 x 1024 x 1280 fp16, 5 vectors in 8 lanes: 134 us, in parts 85).
+    const int maxU = backward ? 2 : one ? 8 : 4;
+    const bool large = !backward && held > 512 * maxU;
+    if (large && ((long long)kg * Cg + V - 1) / V * 4 < 3LL << lc) return false;
+    const int maxT = large || (one && lc == 10) ? 1024 : 512;
     int T = 64;
-    while (T < maxT && (((long long)S << lc) > (long long)T * 2 || T < (1 << lc))) T *= 2;
+    while (T < maxT && (held > (long long)T * 2 || T < (1 << lc))) T *= 2;
     if (T < (1 << lc)) return false;
     const int rows = T >> lc, U = (S + rows - 1) / rows;
     if (U > maxU) return false;
@@ -917,13 +929,13 @@ static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
     p.tiles = (int)(((cvs - 1) >> lc) + 1);
     p.rows = 256 >> lc;
     p.slots = lc > 6 ? p.rows : 4;
-    // 8 positions a thread; 4 or 2 where a sample would have less than 64 workgroups (3 x 1961 x 90 fp32: the backward pass's sums in 7.0 us
-    // against 12.4); more where it would have over 512 parts.  By the sample's own sizes alone: its result is the
-    // same, bit for bit, in a batch of any size.
+    // 8 positions a thread; 4 where a sample would have less than 64 workgroups, 2 where less than 32 (1 x 1961 x 90 fp32, 48 workgroups: 22.0 us a
+    // training pass with 4, 20.7 with 2; 64 x 1961 x 90 79 and 86); more where it would have over 512 parts.  By the sample's own sizes alone: its
+    // result is the same, bit for bit, in a batch of any size.
     long long P = 0;
     for (long long each = 8; each >= 2; each /= 2) {
         P = (S + each * p.rows - 1) / (each * p.rows);
-        if (P * p.tiles >= 64) break;
+        if (P * p.tiles >= 8 * each) break;
     }
     if (P > 512) P = 512;
     p.len = (int)((S + P - 1) / P);
