@@ -706,15 +706,15 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
     }
 }
 
-// A workgroup per (sample, group): the parts of its channels, in order; ab[n][c], and the group's (s1 / M, s2 / M) to coef[n][g].  5.6 us for
-// 128 groups of 8 channels in 512 parts.
-__global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int lcw, const float2* part, float2* ab, float2* coef) {
+// `chunks` workgroups per (sample, group): the parts of its channels, in order; ab[n][c], and the (s1 / M, s2 / M) of a workgroup's channels to
+// coef[n][g][chunk].  5.6 us for 128 groups of 8 channels in 512 parts.
+__global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int lcw, int chunks, const float2* part, float2* ab, float2* coef) {
     __shared__ float2 sh[256];
-    const int n = blockIdx.x / a.G, g = blockIdx.x - n * a.G;
+    const int ng = blockIdx.x / chunks, n = ng / a.G, g = ng - n * a.G;
     const int cw = 1 << lcw, slots = 256 >> lcw, slot = threadIdx.x >> lcw, cl = threadIdx.x & (cw - 1);
     float s1 = 0.f, s2 = 0.f;
-    for (int c0 = 0; c0 < a.Cg; c0 += cw) {
-        const int c = g * a.Cg + c0 + cl;
+    for (long long c0 = (long long)(blockIdx.x - ng * chunks) << lcw; c0 < a.Cg; c0 += (long long)chunks << lcw) {
+        const int c = g * a.Cg + (int)c0 + cl;
         float2 v = make_float2(0.f, 0.f);
         if (c0 + cl < a.Cg) {
             const float2* mine = part + (long long)n * P * a.C + c;
@@ -761,6 +761,21 @@ __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int l
         const float inv = 1.f / ((float)a.S * (float)a.Cg);
         if (threadIdx.x == 0) coef[blockIdx.x] = make_float2(t1 * inv, t2 * inv);
     }
+}
+
+// The chunks of a group, a wave each group: coef[n][g].
+__global__ __launch_bounds__(256) void gn_bwd_coef_kernel(int groups, int chunks, const float2* chunk, float2* coef) {
+    const int id = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= groups) return;
+    float t1 = 0.f, t2 = 0.f;
+    for (int q = threadIdx.x & 63; q < chunks; q += 64) {
+        const float2 o = chunk[(long long)id * chunks + q];
+        t1 += o.x;
+        t2 += o.y;
+    }
+    t1 = wave_sum(t1);
+    t2 = wave_sum(t2);
+    if ((threadIdx.x & 63) == 0) coef[id] = make_float2(t1, t2);
 }
 
 // dw, db: 32 channels a workgroup, 8 lanes a channel share its `rows` partial sums.
@@ -842,12 +857,14 @@ struct GnPlan {
     int U, threads, blocks, walkers;
     size_t lds;
     GnParts p;
-    long long words, ab, coef;       // workspace in floats; offsets of ab[][C] and coef[N][G] in it
+    int lcw, chunks;                 // backward: log2 of the channels, and workgroups a group, that join the parts
+    long long words, ab, coef, chunk;       // workspace in floats; offsets of ab[][C], coef[N][G] and the chunks' in it
 };
 // Vectors of a slab at most.  Forward, 8192 (8 x 4096 x 256 fp16: 17 us, in parts 20; 64 x 1961 x 90 fp32 32 and 35).  Backward, where x and dy
 // are held, 1024: the 2000 vectors of 64 x 2000 x 64 fp16 in 8 groups took 55 us a training pass, 44 in parts, and 24 and 19.5 for one sample.
 #define GN_SLAB_FWD 8192
 #define GN_SLAB_BWD 1024
+#define GN_JOIN_SPLIT 8192
 static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backward) {
     const int Cg = C / G;
     const auto lcols = [&](int k) { return log2_up(((long long)k * Cg + V - 1) / V); };
@@ -945,7 +962,18 @@ static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
     if (backward) {
         r.ab = 2LL * N * p.P * C;
         r.coef = r.ab + 2LL * N * C;
-        r.words = r.coef + 2LL * N * G;
+        r.chunk = r.coef + 2LL * N * G;
+        // One workgroup a group; wide groups in many parts take one per 16 channels (more where the parts are few), and a launch more that adds
+        // those up: 1 x 65536 x 512 bf16 in one group, 512 parts, 200 us a training pass with one workgroup and 114 so, 4 x 4 x 8192 in one group 49
+        // and 23; 65536 x 256 in 32 groups, 4096 sums a group, 70 and 71.
+        r.lcw = log2_up(Cg < 256 ? Cg : 256);
+        r.chunks = 1;
+        if ((long long)Cg * p.P >= GN_JOIN_SPLIT) {
+            const int slots = log2_up((p.P + 7) / 8);
+            r.lcw = 8 - (slots < 4 ? slots : 4);
+            r.chunks = (int)(((long long)Cg + (1 << r.lcw) - 1) >> r.lcw);
+        }
+        r.words = r.chunk + (r.chunks > 1 ? 2LL * N * G * r.chunks : 0);
     } else {
         const long long per = ((long long)V << lc) / Cg + 2;
         const long long groups = per < G ? per : G;
@@ -1015,8 +1043,13 @@ static int run_bwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) 
         const int blocks = a.N * r.p.P * r.p.tiles;
         hipLaunchKernelGGL((gn_bwd_sums_kernel<E, ACT>), dim3(blocks), dim3(256), 0, st, a, r.p, part);
         AG2V_CHECK_LAUNCH();
-        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.N * a.G), dim3(256), 0, st, a, r.p.P, log2_up(a.Cg < 256 ? a.Cg : 256), part, sums, coef);
+        float2* chunk = r.chunks > 1 ? (float2*)(ws + r.chunk) : coef;
+        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.N * a.G * r.chunks), dim3(256), 0, st, a, r.p.P, r.lcw, r.chunks, part, sums, chunk);
         AG2V_CHECK_LAUNCH();
+        if (r.chunks > 1) {
+            hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3(ceil_div((long long)a.N * a.G, 4)), dim3(256), 0, st, a.N * a.G, r.chunks, chunk, coef);
+            AG2V_CHECK_LAUNCH();
+        }
         if (a.y) {
             const int pblocks = params ? ceil_div(a.C, 32) : 0;
             const dim3 grid(blocks + pblocks);
@@ -1046,7 +1079,7 @@ static int run_elem(const GnArgs& a, const GnPlan& r, int act, bool backward, fl
 static int run_any(const GnArgs& a, int dtype, int act, bool backward, float* ws, size_t ws_floats, hipStream_t st) {
     const GnPlan r = plan_of(dtype, a.N, a.S, a.C, a.G, backward);
     if ((r.words && !ws) || ws_floats < (size_t)r.words || ((uintptr_t)ws & 15)) return AG2V_EINVAL;
-    if (!r.slab && (long long)a.N * r.p.P * r.p.tiles >= (1LL << 24)) return AG2V_EINVAL;
+    if (!r.slab && ((long long)a.N * r.p.P * r.p.tiles >= (1LL << 24) || (long long)a.N * a.G * r.chunks >= (1LL << 24))) return AG2V_EINVAL;
     if (dtype == AG2V_F32) return run_elem<ElemF32>(a, r, act, backward, ws, st);
     return dtype == AG2V_BF16 ? run_elem<ElemBF16>(a, r, act, backward, ws, st) : run_elem<ElemF16>(a, r, act, backward, ws, st);
 }

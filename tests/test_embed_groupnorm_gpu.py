@@ -252,6 +252,13 @@ def test_group_norm_act_wide(C, G, device):
         _norm_case(device, (1, 2600, C), G, dtype, 'silu', True, dtype, seed=G)
 
 
+@pytest.mark.parametrize("N,S,C,G", [(2, 4, 8192, 1), (3, 5, 4100, 1), (1, 4096, 256, 2), (2, 1700, 530, 2), (1, 4100, 48, 1), (2, 9000, 96, 1)], ids=str)
+def test_group_norm_act_wide_groups_in_parts(N, S, C, G, device):
+    """Groups whose parts one workgroup joins, or several."""
+    for dtype in (torch.float32, torch.float16):
+        _norm_case(device, (N, S, C), G, dtype, 'silu', True, torch.float32)
+
+
 @pytest.mark.parametrize("C", [64, 90, 112], ids=str)
 def test_group_norm_act_batch_does_not_matter(C, device):
     """y and dx of a sample are the same bits alone and in a batch, also where only the batch is large enough to go past the caches."""
