@@ -875,9 +875,12 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     // training: 16.5 us, two groups 20.2).
     const long long bytes = (long long)S * C * (16 / V) * (backward ? 2 : 1);
     const bool small = bytes <= (1 << 20);
+    // Rows of whole vectors at least, where that is not a matter of a few workgroups: 64 x 930 x 298 bf16 in 149 groups took 150 us forward in rows of
+    // one group, 4 bytes, and takes 55, 64 x 1500 x 64 fp16 in 32 groups 58 and 17 (one sample 9.6 and 11.1); but 600 x 8 fp16 in 4 groups 7.3 and 10.
+    const bool whole = S > 2048 || (long long)S * C * (16 / V) >= 65536;
     int kg = 1;
     while (kg < G && (long long)kg * Cg < 4 * V && lcols(kg + 1) <= 2 && ((long long)S << lcols(kg + 1)) <= most &&
-           !(small && (((long long)S << lcols(kg)) >= 512 || (Cg % V && 4 * Cg >= V)) && (S <= 2048 || (long long)kg * Cg >= V)))
+           !(small && (((long long)S << lcols(kg)) >= 512 ? !whole || (long long)kg * Cg >= V : Cg % V && 4 * Cg >= V)))
         ++kg;
     const int lc = lcols(kg);
     // Narrow rows of a larger map: every cache line would be fetched by many slabs, in pieces (13 x 1085 x 1560 fp16 in 195 groups, one vector a
