@@ -876,11 +876,12 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     const long long bytes = (long long)S * C * (16 / V) * (backward ? 2 : 1);
     const bool small = bytes <= (1 << 20);
     // Rows of whole vectors at least, where that is not a matter of a few workgroups: 64 x 930 x 298 bf16 in 149 groups took 150 us forward in rows of
-    // one group, 4 bytes, and takes 55, 64 x 1500 x 64 fp16 in 32 groups 58 and 17 (one sample 9.6 and 11.1); but 600 x 8 fp16 in 4 groups 7.3 and 10.
+    // one group, 4 bytes, and takes 55, 64 x 1500 x 64 fp16 in 32 groups 58 and 17 (one sample 9.6 and 11.1), 64 x 480 x 300 bf16 in 100 groups 80 and
+    // 47 (one sample 7.9 and 10.2); but 600 x 8 fp16 in 4 groups 7.3 and 10.
     const bool whole = S > 2048 || (long long)S * C * (16 / V) >= 65536;
     int kg = 1;
     while (kg < G && (long long)kg * Cg < 4 * V && lcols(kg + 1) <= 2 && ((long long)S << lcols(kg + 1)) <= most &&
-           !(small && (((long long)S << lcols(kg)) >= 512 ? !whole || (long long)kg * Cg >= V : Cg % V && 4 * Cg >= V)))
+           !(small && (((long long)S << lcols(kg)) >= 512 || (Cg % V && 4 * Cg >= V)) && (!whole || (long long)kg * Cg >= V)))
         ++kg;
     const int lc = lcols(kg);
     // Narrow rows of a larger map: every cache line would be fetched by many slabs, in pieces (13 x 1085 x 1560 fp16 in 195 groups, one vector a
@@ -889,8 +890,9 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     if (kg < G && (long long)kg * Cg < V && S > 2048) return false;
     const long long held = (long long)S << lc;
     if (!small && kg < G && !backward && (long long)kg * Cg < 2 * V && Cg % V) return false;
-    // Backward they are, beyond 512 vectors in rows of up to 32 bytes also on small maps: 64 x 1024 x 256 bf16 in 32 groups took 87 us a training pass, 71 in parts (one sample
-    // 18.8 and 19.1), and 64 x 1000 x 50 fp16 in 10 groups 61 and 46.  Rows of 60 are not: 200 x 90 fp32 in 6 groups 14.3 and 15.6.
+    // Backward they are, beyond 512 vectors in rows of up to 32 bytes also on small maps: 64 x 1024 x 256 bf16 in 32 groups took 87 us a training
+    // pass, 71 in parts (one sample 18.8 and 19.1), and 64 x 1000 x 50 fp16 in 10 groups 61 and 46.  Rows of 60 are not: 200 x 90 fp32 in 6 groups
+    // 14.3 and 15.6.
     if (kg < G && backward && ((!small && (long long)kg * Cg < 4 * V) || (held > 512 && (long long)kg * Cg <= 2 * V))) return false;
     if (lc > 10 || held > most) return false;
     const bool one = kg == 1 || Cg % V == 0;

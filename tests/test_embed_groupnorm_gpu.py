@@ -259,6 +259,13 @@ def test_group_norm_act_wide_groups_in_parts(N, S, C, G, device):
         _norm_case(device, (N, S, C), G, dtype, 'silu', True, torch.float32)
 
 
+@pytest.mark.parametrize("S,C,G", [(300, 6, 3), (93, 298, 149), (930, 298, 149), (480, 300, 100), (513, 48, 16), (400, 62, 31), (1025, 34, 17), (515, 66, 22)], ids=str)
+def test_group_norm_act_narrow_groups(S, C, G, device):
+    """Groups of a few channels: one of them, or as many as fill a vector, side by side in a workgroup."""
+    for dtype in (torch.float32, torch.bfloat16):
+        _norm_case(device, (2, S, C), G, dtype, 'lrelu', True, dtype)
+
+
 @pytest.mark.parametrize("C", [64, 90, 112], ids=str)
 def test_group_norm_act_batch_does_not_matter(C, device):
     """y and dx of a sample are the same bits alone and in a batch, also where only the batch is large enough to go past the caches."""
