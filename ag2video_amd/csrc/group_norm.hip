@@ -320,7 +320,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
             for (int k = 0; k < V; ++k) {
                 A[k] += sA[k];
                 B[k] += sB[k];
-                if (k >= dup) {
+                if (k >= dup && at + k < W) {      // (w and b behind W are the next group's)
                     g1[k % NG] = fmaf(w[k], sA[k], g1[k % NG]);
                     g2[k % NG] = fmaf(w[k], sB[k], g2[k % NG]);
                 }
