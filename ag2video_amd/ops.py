@@ -2329,7 +2329,8 @@ def embedding_scaled(idx, table, scale=1.0, padding_idx=None):
     Gradient: scale * (sum of the result's gradient rows by token), in fp32, rounded once, with a fixed order of summation (no atomics);
     the row ``padding_idx`` gets none.  The tokens are sorted, so the work is that of one pass over the gradient rows and the table,
     whatever the vocabulary.  A token outside [0, V) cannot be refused without waiting for the device: its row comes back as NaN, it adds
-    to no gradient, and nothing outside the table is read.  No second derivative (a backward pass with create_graph=True is refused)."""
+    to no gradient, and nothing outside the table is read.  No second derivative (a backward pass with create_graph=True is refused) and no
+    forward-mode one (a dual table is refused)."""
     return _lib.elem_ops().embedding_scaled(idx, table, scale, padding_idx)
 
 
@@ -2341,8 +2342,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act='silu', slop
     channels are adjacent are read in place (a channel slice; ``t.permute(0, 2, 3, 1)`` of a channels-last NCHW tensor).  Gradients for x,
     weight and bias; h and the activation's derivative are computed again from x, so the tape holds x and two numbers per group.  Sums in
     fp32 in a fixed order (no atomics); y and dx of a sample do not depend on the rest of the batch.  No second
-    derivative (a backward pass with create_graph=True is refused).  Fewer than 2^24 (sample, group) pairs,
-    2^30 positions and channels."""
+    derivative (a backward pass with create_graph=True is refused) and no forward-mode one (dual inputs are refused).  Fewer than 2^24
+    (sample, group) pairs, 2^30 positions and channels."""
     return _lib.elem_ops().group_norm_act(x, groups, weight, bias, eps, act, slope)
 
 
