@@ -4,7 +4,8 @@
 //     z = w h + b                y = act(z):  0 z,  1 z * sigmoid(z),  2 z > 0 ? z : slope * z
 //   backward, dz = dy act'(z), A[n,c] = sum_s dz, B[n,c] = sum_s dz h:
 //     db = sum_n A, dw = sum_n B, s1 = sum_{c in g} w A, s2 = sum_{c in g} w B, dx = rstd (w dz - (s1 + h s2) / M)
-// Every sum is in fp32; z and h are computed again in the backward pass from x and the two statistics of a group.
+// Every sum is in fp32; z and h are computed again in the backward pass from x and the two statistics of a group: h as written, because the
+// rounding of mean * rstd in x * rstd - mean * rstd would be one of |mean| rstd 2^-24 in h, more than all else where the mean is far from zero.
 //
 // Memory bounds all of it: forward x is read and y written, backward x and dy are read and dx written.  A (sample, set of groups) that fits
 // the registers of a workgroup is read once, in one launch (gn_slab_*).  A larger one is read twice: parts of a sample's positions give
@@ -296,11 +297,11 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
                 rd[u] = load_vec<E>(dy + r * a.dr, W);
             }
         }
-        float off[NG], rstd[NG], sA[V] = {}, sB[V] = {}, g1[NG] = {}, g2[NG] = {};      // h = x rstd + off; sums of dz, dz h; of w dz, w dz h
+        float mean[NG], rstd[NG], sA[V] = {}, sB[V] = {}, g1[NG] = {}, g2[NG] = {};      // sums of dz, dz h; of w dz, w dz h
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
             rstd[k] = here ? a.rstd[(long long)n * a.G + g0 + gi[k]] : 0.f;
-            off[k] = here ? -a.mean[(long long)n * a.G + g0 + gi[k]] * rstd[k] : 0.f;
+            mean[k] = here ? a.mean[(long long)n * a.G + g0 + gi[k]] : 0.f;
         }
         if (here) {
 #pragma unroll
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = fmaf(v[k], rstd[k % NG], off[k % NG]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                        const float h = (v[k] - mean[k % NG]) * rstd[k % NG], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                         sA[k] += dz;
                         sB[k] = fmaf(dz, h, sB[k]);
                     }
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = fmaf(v[k], rstd[k % NG], off[k % NG]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                        const float h = (v[k] - mean[k % NG]) * rstd[k % NG], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                         v[k] = rstd[k % NG] * (w[k] * dz - g1[k % NG] - h * g2[k % NG]);
                     }
                     store_tail<E>(dx + (long long)r * a.C, dup, W, v);
@@ -653,12 +654,10 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
     const int cols = 1 << p.lc, width = cols * V;
     float A[V] = {}, B[V] = {};
     if (i.on) {
-        float off[V], rstd[V], w[V], b[V];
+        float mean[V], rstd[V], w[V], b[V];
         load_params<E>(a.w, a.ptype, i.c, a.C, 1.f, w);
         load_params<E>(a.b, a.ptype, i.c, a.C, 0.f, b);
-        load_stats<V>(a, i.n, i.c, off, rstd);
-#pragma unroll
-        for (int k = 0; k < V; ++k) off[k] = -off[k] * rstd[k];
+        load_stats<V>(a, i.n, i.c, mean, rstd);
         const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
         const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c;
         for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
@@ -677,7 +676,7 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = fmaf(v[k], rstd[k], off[k]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                        const float h = (v[k] - mean[k]) * rstd[k], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                         A[k] += dz;
                         B[k] = fmaf(dz, h, B[k]);
                     }
@@ -813,13 +812,11 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
     }
     const GnWhere i = where_of<V>(a, p, blockIdx.x - pblocks);
     if (!i.on) return;
-    float off[V], rstd[V], w[V], b[V];
+    float mean[V], rstd[V], w[V], b[V];
     float2 cf[V];
     load_params<E>(a.w, a.ptype, i.c, a.C, 1.f, w);
     load_params<E>(a.b, a.ptype, i.c, a.C, 0.f, b);
-    load_stats<V>(a, i.n, i.c, off, rstd, coef, cf);
-#pragma unroll
-    for (int k = 0; k < V; ++k) off[k] = -off[k] * rstd[k];
+    load_stats<V>(a, i.n, i.c, mean, rstd, coef, cf);
     const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
     const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c;
     typename E::T* dx = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c;
@@ -839,7 +836,7 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
                 E::unpack(rd[u], d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    const float h = fmaf(v[k], rstd[k], off[k]), dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                    const float h = (v[k] - mean[k]) * rstd[k], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
                     v[k] = rstd[k] * (w[k] * dz - cf[k].x - h * cf[k].y);
                 }
                 store_tail<E, NT != 0>(dx + (long long)(r + u * p.rows) * a.C, i.dup, a.C, v);

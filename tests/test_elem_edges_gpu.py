@@ -46,3 +46,66 @@ def test_parameters_that_are_not_finite_stay_in_their_group(Cg, S, dtype, device
             own[c] = False
             for name, q, r in zip(('y', 'dweight', 'dbias'), (got[0], got[2], got[3]), (want[0], want[2], want[3])):
                 assert torch.equal(q[..., own], r[..., own]), (name, act, which, value)
+
+
+# Maps on which a group's mean is exact: sums of numbers of few bits, counts that are powers of two, values on both sides of the mean in pairs.  One
+# launch and parts.
+EXACT = [((2, 64, 16), 4), ((2, 64, 6), 3), ((2, 512, 8), 8), ((1, 16384, 16), 2), ((2, 8192, 64), 4)]
+
+
+@pytest.mark.parametrize("shape,G", EXACT, ids=str)
+def test_constant_groups_far_from_zero(shape, G, device):
+    """x = mean exactly: h = 0, y = act(b), dweight = 0."""
+    C = shape[-1]
+    for value in (3.25, 1000.125, -31007.5):
+        x = torch.full(shape, value)
+        w, b, dy = 1 + 0.2 * _randn(C, seed=1), _randn(C, seed=2), _randn(*shape, seed=3)
+        y, dx, dw, db = _norm_all(device, x, G, w, b, dy, 'silu')
+        # fma(0, w, b) = b; the sigmoid from exp and a reciprocal: (4 + |z|) u relative, and the product
+        want = b.double() * torch.sigmoid(b.double())
+        assert ((y.double() - want).abs() <= (5 + b.double().abs()) * R.U * want.abs()).all()
+        assert not dw.any()
+
+
+@pytest.mark.parametrize("act", ['none', 'silu'])
+@pytest.mark.parametrize("shape,G", EXACT, ids=str)
+def test_gradients_far_from_zero(shape, G, act, device):
+    """Values around 1000 whose mean is exact: the backward pass has h to a few roundings of h itself, not of |mean| / std.
+
+    x - mean is exact, so h carries the relative error of 1 / std (the variance: at most DEPTH additions of positive terms; four more for the division, the
+    root and the reciprocal) and of one product: e_h = |h| (DEPTH / 2 + 5) u.  In parts the statistics are joined in fp64, which adds less.  What
+    follows from e_h is as in _elem_ref.group_norm."""
+    N, S, C = shape
+    Cg = C // G
+    off = _randn(N, S, C, seed=1).mul(8).round().clamp(-40, 40) / 16
+    if Cg == 1:                                               # symmetric: the mean of a group is 1000, exactly
+        off[:, S // 2:] = -off[:, :S // 2]
+    else:
+        off[..., 1::2] = -off[..., ::2]
+    x = 1000 + off
+    w, b, dy = 1 + 0.2 * _randn(C, seed=3), _randn(C, seed=4), 1 + 0.1 * _randn(*shape, seed=5)
+    y, dx, dw, db = _norm_all(device, x, G, w, b, dy, act)
+    v = x.double().view(N, S, G, Cg)
+    d = v - 1000.0
+    rstd = ((d * d).mean((1, 3), keepdim=True) + 1e-5) ** -0.5
+    r_rstd = (R.DEPTH / 2 + 4) * R.U
+    h, e_h = d * rstd, (d * rstd).abs() * (r_rstd + R.U)
+    wd, bd, g = w.double().view(1, 1, G, Cg), b.double().view(1, 1, G, Cg), dy.double().view(v.shape)
+    z = h * wd + bd
+    e_z = wd.abs() * e_h + 3 * R.U * ((wd * h).abs() + bd.abs())
+    if act == 'silu':
+        s = torch.sigmoid(z)
+        dz, e_dz = g * s * (1 + z * (1 - s)), g.abs() * (0.5 * e_z + (8 + 2 * z.abs()) * R.U * (1 + z.abs()))
+    else:
+        dz, e_dz = g, torch.zeros_like(g)
+    du = R.DEPTH * R.U
+    total, err = (dz * h).sum((0, 1)).view(-1), (e_dz * h.abs() + dz.abs() * e_h + (2 * du + R.U) * (dz * h).abs()).sum((0, 1)).view(-1)
+    R.check('dweight', dw, total, err + R.U * (total.abs() + err))
+    t, e_t = wd * dz, wd.abs() * e_dz + R.U * (wd * dz).abs()
+    dims = (1, 3)
+    s1, s2 = t.mean(dims, keepdim=True), (t * h).mean(dims, keepdim=True)
+    e_s1 = e_t.mean(dims, keepdim=True) + (du + 2 * R.U) * t.abs().mean(dims, keepdim=True)
+    e_s2 = (e_t * h.abs() + t.abs() * e_h + R.U * (t * h).abs()).mean(dims, keepdim=True) + (du + 2 * R.U) * (t * h).abs().mean(dims, keepdim=True)
+    ref = rstd * (t - s1 - h * s2)
+    bound = rstd * (e_t + e_s1 + h.abs() * e_s2 + s2.abs() * e_h + 4 * R.U * (t.abs() + s1.abs() + (h * s2).abs())) + ref.abs() * (r_rstd + 2 * R.U)
+    R.check('dx', dx.view(v.shape), ref, bound + R.U * (ref.abs() + bound))
