@@ -720,6 +720,7 @@ static int log2_up(long long v) {
 }
 static int vec_of(int dtype) { return dtype == AG2V_F32 ? ElemF32::V : ElemBF16::V; }
 
+#define MOST_BLOCKS (1LL << 24)     // a launch takes fewer than 2^32 threads: fewer workgroups of 256 than this
 // How the gradient of (n, V, D) runs.
 struct EmbedPlan {
     bool pick, tile, rank;
@@ -744,13 +745,16 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
     // have a counter each in LDS
     p.T = TILE_MIN;
     while (p.T < TILE_MAX && n >= 512LL * p.T) p.T *= 2;
-    p.tile = V * 16 <= (dtype == AG2V_F32 ? 4 : 2) * p.T && V < 1 << TILE_BITS && n <= 512LL * TILE_MAX;
+    // (rows so wide that their slices would pass what a launch holds go the other way)
+    const long long slices16 = (cv + 15) >> 4;
+    p.tile = V * 16 <= (dtype == AG2V_F32 ? 4 : 2) * p.T && V < 1 << TILE_BITS && n <= 512LL * TILE_MAX && slices16 * V < MOST_BLOCKS / 4 &&
+             slices16 * ((n + p.T - 1) / p.T) < MOST_BLOCKS / 4;
     if (p.tile) {
         p.jlsh = p.lsh;
         p.jslices = p.slices;
         if (p.lsh > 4) {                // 16 lanes a row: shares of 16 tokens at least, and more workgroups
             p.lsh = 4;
-            p.slices = (int)((cv + 15) >> 4);
+            p.slices = (int)slices16;
         }
         p.tiles = (int)((n + p.T - 1) / p.T);
         if (p.tiles > TILE_JOIN_WIDE) {
@@ -765,11 +769,11 @@ static EmbedPlan plan_of(int dtype, long long n, long long V, int D) {
     // two or more from about 11000
     p.rank = n <= (V < RADIX_N ? RANK_MAX * 3 / 4 : RANK_MAX);
     // entries a group walks: enough groups for 4096 waves, 8 .. 64 (for 2048 waves 131072 rows of 389 fp16 take 49 us and not 37; for 8192 the join
-    // of their longest segment 14 us and not 8.6); more only where the workgroups' parts would pass 16384
+    // of their longest segment 14 us and not 8.6); more only where the workgroups' parts would pass 16384, or the workgroups what a launch holds
     const int ng = 256 >> p.lsh;
     long long L = (n * p.slices << p.lsh) / 64 / 4096;
     L = L < 8 ? 8 : L > 64 ? 64 : 1LL << (log2_up(L + 1) - 1);
-    while ((n + ng * L - 1) / (ng * L) > 16384) L *= 2;
+    while ((n + ng * L - 1) / (ng * L) > 16384 || (n + ng * L - 1) / (ng * L) * p.slices >= MOST_BLOCKS) L *= 2;
     p.L = (int)L;
     p.nblk = (int)((n + ng * L - 1) / (ng * L));
     p.npad = (n + 63) / 64 * 64;
@@ -886,7 +890,6 @@ extern "C" int ag2v_embed_bwd(int dtype, const void* idx, int idx_bytes, long lo
     if (!idx || !dout || !dtable || !embed_ok(dtype, idx_bytes, n, V, D)) return AG2V_EINVAL;
     const EmbedPlan p = plan_of(dtype, n, V, D);
     if ((p.words && !workspace) || workspace_floats < (size_t)p.words || ((uintptr_t)workspace & 15)) return AG2V_EINVAL;
-    if ((long long)p.nblk * p.slices >= (1LL << 24)) return AG2V_EINVAL;
     const int wide = idx_bytes == 8, pad = padding_idx >= 0 && padding_idx < V ? (int)padding_idx : -1;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == AG2V_F32)

@@ -777,29 +777,33 @@ __global__ __launch_bounds__(256) void gn_bwd_coef_kernel(int groups, int chunks
     if ((threadIdx.x & 63) == 0) coef[id] = make_float2(t1, t2);
 }
 
-// dw, db: 32 channels a workgroup, 8 lanes a channel share its `rows` partial sums.
-__device__ __forceinline__ void params_of(const GnArgs& a, int blk, int rows, const float2* ab) {
+// dw, db: 32 channels a workgroup at a time, 8 lanes a channel share its `rows` partial sums.
+__device__ __forceinline__ void params_of(const GnArgs& a, int blk, int nblk, int rows, const float2* ab) {
     __shared__ float2 sh[256];
-    const int cl = threadIdx.x & 31, slot = threadIdx.x >> 5, c = blk * 32 + cl;
-    float2 v = make_float2(0.f, 0.f);
-    if (c < a.C)
-        for (int r = slot; r < rows; r += 8) {
-            const float2 o = ab[(long long)r * a.C + c];
-            v.x += o.x;
-            v.y += o.y;
+    const int cl = threadIdx.x & 31, slot = threadIdx.x >> 5;
+    for (int c0 = blk * 32; c0 < a.C; c0 += nblk * 32) {
+        const int c = c0 + cl;
+        float2 v = make_float2(0.f, 0.f);
+        if (c < a.C)
+            for (int r = slot; r < rows; r += 8) {
+                const float2 o = ab[(long long)r * a.C + c];
+                v.x += o.x;
+                v.y += o.y;
+            }
+        sh[threadIdx.x] = v;
+        __syncthreads();
+        if (slot == 0 && c < a.C) {
+            for (int q = 1; q < 8; ++q) {
+                v.x += sh[q * 32 + cl].x;
+                v.y += sh[q * 32 + cl].y;
+            }
+            if (a.dw) store_any(a.dw, a.ptype, c, v.y);
+            if (a.db) store_any(a.db, a.ptype, c, v.x);
         }
-    sh[threadIdx.x] = v;
-    __syncthreads();
-    if (slot == 0 && c < a.C) {
-        for (int q = 1; q < 8; ++q) {
-            v.x += sh[q * 32 + cl].x;
-            v.y += sh[q * 32 + cl].y;
-        }
-        if (a.dw) store_any(a.dw, a.ptype, c, v.y);
-        if (a.db) store_any(a.db, a.ptype, c, v.x);
+        __syncthreads();
     }
 }
-__global__ __launch_bounds__(256) void gn_params_kernel(GnArgs a, int rows, const float2* ab) { params_of(a, blockIdx.x, rows, ab); }
+__global__ __launch_bounds__(256) void gn_params_kernel(GnArgs a, int rows, const float2* ab) { params_of(a, blockIdx.x, gridDim.x, rows, ab); }
 
 // dx; the first `pblocks` workgroups sum the parameters' gradients instead.  NT: 1 stores past the caches, 2 loads too.  403 MB (4 x 65536 x 256
 // bf16) in 66 us, 6.1 TB/s: memory.
@@ -807,7 +811,7 @@ template <class E, int ACT, int NT>
 __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef, int pblocks, const float2* ab) {
     constexpr int V = E::V, U = 4;
     if ((int)blockIdx.x < pblocks) {
-        params_of(a, blockIdx.x, a.N, ab);
+        params_of(a, blockIdx.x, pblocks, a.N, ab);
         return;
     }
     const GnWhere i = where_of<V>(a, p, blockIdx.x - pblocks);
@@ -847,11 +851,17 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
 // ---------------------------------------------------------------- host
 static int vec_of(int dtype) { return dtype == AG2V_F32 ? ElemF32::V : ElemBF16::V; }
 
-// Which way (N, S, C, G) runs, forward or backward.
+// A launch takes fewer than 2^32 threads in all.  Batches that need more workgroups go by several launches of `per` samples.
+#define GN_SLAB_BLOCKS ((1 << 22) - 1)      // of up to 1024 threads
+#define GN_BLOCKS ((1 << 23) - 1)           // of 256, and beside as many again
+#define GN_PARAM_BLOCKS (1 << 20)
+// Which way (S, C, G) runs, forward or backward, and what N samples need.  Nothing but `per`, the walkers and the workspace depends on N: a sample's
+// result is the same, bit for bit, in a batch of any size.
 struct GnPlan {
     bool slab, one, join_here;      // one: a vector lies inside one group; join_here: the second pass joins the parts itself
     GnSlab s;
-    int U, threads, blocks, walkers;
+    int U, threads, walkers;
+    int per;                         // samples a launch
     size_t lds;
     GnParts p;
     int lcw, chunks;                 // backward: log2 of the channels, and workgroups a group, that join the parts
@@ -917,22 +927,21 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     r.s.slots = lc > 6 ? rows : T / 64;
     r.s.wg = kg == 1 && one ? 1 << lc : one ? Cg / V : Cg;
     r.s.llg = share_lanes(T, kg);
-    r.s.nslab = (long long)N * r.s.nsets;
     const int subs = r.threads / T;
     r.lds = sizeof(float) * subs * (((size_t)r.s.slots << lc) * (backward ? (one ? V : 2 * V) : (one ? 1 : V)) + 2 * kg);
-    long long blocks;
+    if (r.s.nsets > GN_SLAB_BLOCKS || r.lds > 64 * 1024) return false;
+    r.per = N;
     if (!backward) {
-        blocks = (r.s.nslab + subs - 1) / subs;
-    } else {
+        const long long per = (long long)GN_SLAB_BLOCKS * subs / r.s.nsets;
+        if (per < N) r.per = (int)per;
+    } else {                             // (any number of samples in one launch)
         long long wb = ((long long)N + subs - 1) / subs;
         const long long cap = 2048 / r.s.nsets < 1 ? 1 : 2048 / r.s.nsets;
         if (wb > cap) wb = cap;
         r.walkers = (int)wb * subs;
-        blocks = wb * r.s.nsets;
         r.words = 2LL * r.walkers * C;
     }
-    r.blocks = (int)blocks;
-    return blocks < (1LL << 22) && r.lds <= 64 * 1024;
+    return true;
 }
 static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
     GnPlan r = {};
@@ -949,22 +958,20 @@ static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
     p.rows = 256 >> lc;
     p.slots = lc > 6 ? p.rows : 4;
     // 8 positions a thread; 4 where a sample would have less than 64 workgroups, 2 where less than 32 (1 x 1961 x 90 fp32, 48 workgroups: 22.0 us a
-    // training pass with 4, 20.7 with 2; 64 x 1961 x 90 79 and 86); more where it would have over 512 parts.  By the sample's own sizes alone: its
-    // result is the same, bit for bit, in a batch of any size.
+    // training pass with 4, 20.7 with 2; 64 x 1961 x 90 79 and 86); more where it would have over 512 parts, or more workgroups than a launch takes.
     long long P = 0;
     for (long long each = 8; each >= 2; each /= 2) {
         P = (S + each * p.rows - 1) / (each * p.rows);
         if (P * p.tiles >= 8 * each) break;
     }
     if (P > 512) P = 512;
+    while (P > 1 && P * p.tiles > GN_BLOCKS) P /= 2;
     p.len = (int)((S + P - 1) / P);
     p.P = (S + p.len - 1) / p.len;
     p.tg = (int)(((long long)Cg - 1) / (V << lc) + 2);
     if (p.tg > p.tiles) p.tg = p.tiles;
+    long long per = GN_BLOCKS / ((long long)p.P * p.tiles);
     if (backward) {
-        r.ab = 2LL * N * p.P * C;
-        r.coef = r.ab + 2LL * N * C;
-        r.chunk = r.coef + 2LL * N * G;
         // One workgroup a group; wide groups in many parts take one per 16 channels (more where the parts are few), and a launch more that adds
         // those up: 1 x 65536 x 512 bf16 in one group, 512 parts, 200 us a training pass with one workgroup and 114 so, 4 x 4 x 8192 in one group 49
         // and 23; 65536 x 256 in 32 groups, 4096 sums a group, 70 and 71.
@@ -973,15 +980,23 @@ static GnPlan plan_of(int dtype, int N, int S, int C, int G, bool backward) {
         if ((long long)Cg * p.P >= GN_JOIN_SPLIT) {
             const int slots = log2_up((p.P + 7) / 8);
             r.lcw = 8 - (slots < 4 ? slots : 4);
-            r.chunks = (int)(((long long)Cg + (1 << r.lcw) - 1) >> r.lcw);
+            const long long most = GN_BLOCKS / G < 1 ? 1 : GN_BLOCKS / G, chunks = ((long long)Cg + (1 << r.lcw) - 1) >> r.lcw;
+            r.chunks = (int)(chunks < most ? chunks : most);
         }
-        r.words = r.chunk + (r.chunks > 1 ? 2LL * N * G * r.chunks : 0);
+        const long long joins = 2LL * GN_BLOCKS / ((long long)G * r.chunks);
+        if (joins < per) per = joins < 1 ? 1 : joins;
+        r.per = per < N ? (int)per : N;
+        r.ab = 2LL * r.per * p.P * C;
+        r.coef = r.ab + 2LL * N * C;
+        r.chunk = r.coef + 2LL * r.per * G;
+        r.words = r.chunk + (r.chunks > 1 ? 2LL * r.per * G * r.chunks : 0);
     } else {
+        r.per = per < N ? (int)per : N;
         const long long per = ((long long)V << lc) / Cg + 2;
         const long long groups = per < G ? per : G;
         p.llg = share_lanes(256, (int)groups);
         r.join_here = groups <= GN_JOIN_GROUPS && groups * p.P * p.tg <= 2048;
-        r.words = 4LL * N * G * p.P * p.tg;
+        r.words = 4LL * r.per * G * p.P * p.tg;
     }
     return r;
 }
@@ -993,26 +1008,43 @@ static bool past_caches(const GnArgs& a) {
     return (long long)a.N * a.S * a.C * (long long)sizeof(typename E::T) > AG2V_NT_STORE_BYTES && a.C * (long long)sizeof(typename E::T) % 64 == 0;
 }
 
+// `count` samples from n0 on
+template <class E>
+static GnArgs samples_of(const GnArgs& a, int n0, int count) {
+    typedef typename E::T T;
+    GnArgs b = a;
+    b.x = (const T*)a.x + n0 * a.xs;
+    if (a.dy) b.dy = (const T*)a.dy + n0 * a.ds;
+    if (a.y) b.y = (T*)a.y + (long long)n0 * a.S * a.C;
+    b.mean = a.mean + (long long)n0 * a.G;
+    b.rstd = a.rstd + (long long)n0 * a.G;
+    b.N = a.N - n0 < count ? a.N - n0 : count;
+    return b;
+}
+
 template <class E, int ACT, bool ONE>
 static int run_slab_fwd(const GnArgs& a, const GnPlan& r, hipStream_t st) {
-    const dim3 grid(r.blocks), block(r.threads);
-    if (r.U == 1) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 1, ONE>), grid, block, r.lds, st, a, r.s);
-    else if (r.U == 2) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 2, ONE>), grid, block, r.lds, st, a, r.s);
-    else if (r.U == 4 || !ONE) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 4, ONE>), grid, block, r.lds, st, a, r.s);
-    else if constexpr (ONE) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 8, true>), grid, block, r.lds, st, a, r.s);
+    GnSlab s = r.s;
+    s.nslab = (long long)a.N * s.nsets;
+    const int subs = r.threads / s.T;
+    const dim3 grid(ceil_div(s.nslab, subs)), block(r.threads);
+    if (r.U == 1) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 1, ONE>), grid, block, r.lds, st, a, s);
+    else if (r.U == 2) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 2, ONE>), grid, block, r.lds, st, a, s);
+    else if (r.U == 4 || !ONE) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 4, ONE>), grid, block, r.lds, st, a, s);
+    else if constexpr (ONE) hipLaunchKernelGGL((gn_slab_fwd_kernel<E, ACT, 8, true>), grid, block, r.lds, st, a, s);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
 template <class E, int ACT, bool ONE>
 static int run_slab_bwd(const GnArgs& a, const GnPlan& r, float2* ab, hipStream_t st) {
-    const dim3 grid(r.blocks), block(r.threads);
+    const dim3 grid(r.walkers / (r.threads / r.s.T) * r.s.nsets), block(r.threads);
     if (r.U == 1) hipLaunchKernelGGL((gn_slab_bwd_kernel<E, ACT, 1, ONE>), grid, block, r.lds, st, a, r.s, r.walkers, ab);
     else hipLaunchKernelGGL((gn_slab_bwd_kernel<E, ACT, 2, ONE>), grid, block, r.lds, st, a, r.s, r.walkers, ab);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
 template <class E, int ACT>
-static int run_fwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) {
+static int run_fwd(const GnArgs& a, const GnPlan& r, bool past, float* ws, hipStream_t st) {
     if (r.slab) return r.one ? run_slab_fwd<E, ACT, true>(a, r, st) : run_slab_fwd<E, ACT, false>(a, r, st);
     const int blocks = a.N * r.p.P * r.p.tiles;
     hipLaunchKernelGGL(gn_stats_kernel<E>, dim3(blocks), dim3(256), 0, st, a, r.p, (float4*)ws);
@@ -1023,65 +1055,80 @@ static int run_fwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) 
         AG2V_CHECK_LAUNCH();
         part = nullptr;
     }
-    if (past_caches<E>(a))
+    if (past)
         hipLaunchKernelGGL((gn_apply_kernel<E, ACT, true>), dim3(blocks), dim3(256), 0, st, a, r.p, part);
     else
         hipLaunchKernelGGL((gn_apply_kernel<E, ACT, false>), dim3(blocks), dim3(256), 0, st, a, r.p, part);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
+static int run_params(const GnArgs& a, int rows, const float2* ab, hipStream_t st) {
+    const int blocks = ceil_div(a.C, 32);
+    hipLaunchKernelGGL(gn_params_kernel, dim3(blocks < GN_PARAM_BLOCKS ? blocks : GN_PARAM_BLOCKS), dim3(256), 0, st, a, rows, ab);
+    AG2V_CHECK_LAUNCH();
+    return AG2V_OK;
+}
+// Backward in parts: sums[n][C] of the samples of `a`; dx, and beside it the parameters' gradients where `params`.
 template <class E, int ACT>
-static int run_bwd(const GnArgs& a, const GnPlan& r, float* ws, hipStream_t st) {
+static int run_bwd_parts(const GnArgs& a, const GnPlan& r, bool past, bool params, float2* sums, float* ws, hipStream_t st) {
+    float2 *part = (float2*)ws, *coef = (float2*)(ws + r.coef);
+    const int blocks = a.N * r.p.P * r.p.tiles;
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<E, ACT>), dim3(blocks), dim3(256), 0, st, a, r.p, part);
+    AG2V_CHECK_LAUNCH();
+    float2* chunk = r.chunks > 1 ? (float2*)(ws + r.chunk) : coef;
+    hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.N * a.G * r.chunks), dim3(256), 0, st, a, r.p.P, r.lcw, r.chunks, part, sums, chunk);
+    AG2V_CHECK_LAUNCH();
+    if (r.chunks > 1) {
+        hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3(ceil_div((long long)a.N * a.G, 4)), dim3(256), 0, st, a.N * a.G, r.chunks, chunk, coef);
+        AG2V_CHECK_LAUNCH();
+    }
+    if (!a.y) return params ? run_params(a, a.N, sums, st) : AG2V_OK;
+    const int all = params ? ceil_div(a.C, 32) : 0, pblocks = all < GN_PARAM_BLOCKS ? all : GN_PARAM_BLOCKS;
+    const dim3 grid(blocks + pblocks);
+    if (past && r.p.tiles == 1)      // (x and dy together pass the bound of loads; the lines of a tiled row are read twice)
+        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 2>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+    else if (past)
+        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 1>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+    else
+        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 0>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+    AG2V_CHECK_LAUNCH();
+    return AG2V_OK;
+}
+template <class E, int ACT>
+static int run_bwd(const GnArgs& a, const GnPlan& r, bool past, float* ws, hipStream_t st) {
     const bool params = a.dw || a.db;
-    int rows = a.N;
-    const float2* ab = (const float2*)ws;
     if (r.slab) {
         float2* out = params ? (float2*)ws : nullptr;
         const int rc = r.one ? run_slab_bwd<E, ACT, true>(a, r, out, st) : run_slab_bwd<E, ACT, false>(a, r, out, st);
-        if (rc != AG2V_OK) return rc;
-        rows = r.walkers;
-    } else {
-        float2 *part = (float2*)ws, *sums = (float2*)(ws + r.ab), *coef = (float2*)(ws + r.coef);
-        const int blocks = a.N * r.p.P * r.p.tiles;
-        hipLaunchKernelGGL((gn_bwd_sums_kernel<E, ACT>), dim3(blocks), dim3(256), 0, st, a, r.p, part);
-        AG2V_CHECK_LAUNCH();
-        float2* chunk = r.chunks > 1 ? (float2*)(ws + r.chunk) : coef;
-        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(a.N * a.G * r.chunks), dim3(256), 0, st, a, r.p.P, r.lcw, r.chunks, part, sums, chunk);
-        AG2V_CHECK_LAUNCH();
-        if (r.chunks > 1) {
-            hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3(ceil_div((long long)a.N * a.G, 4)), dim3(256), 0, st, a.N * a.G, r.chunks, chunk, coef);
-            AG2V_CHECK_LAUNCH();
-        }
-        if (a.y) {
-            const int pblocks = params ? ceil_div(a.C, 32) : 0;
-            const dim3 grid(blocks + pblocks);
-            if (past_caches<E>(a) && r.p.tiles == 1)      // (x and dy together pass the bound of loads; the lines of a tiled row are read twice)
-                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 2>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
-            else if (past_caches<E>(a))
-                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 1>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
-            else
-                hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 0>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
-            AG2V_CHECK_LAUNCH();
-            return AG2V_OK;
-        }
-        ab = sums;
+        return rc != AG2V_OK || !params ? rc : run_params(a, r.walkers, out, st);
     }
-    if (params) {
-        hipLaunchKernelGGL(gn_params_kernel, dim3(ceil_div(a.C, 32)), dim3(256), 0, st, a, rows, ab);
-        AG2V_CHECK_LAUNCH();
+    float2* sums = (float2*)(ws + r.ab);
+    if (r.per == a.N) return run_bwd_parts<E, ACT>(a, r, past, params, sums, ws, st);
+    for (int n0 = 0; n0 < a.N; n0 += r.per) {
+        const int rc = run_bwd_parts<E, ACT>(samples_of<E>(a, n0, r.per), r, past, false, sums + (long long)n0 * a.C, ws, st);
+        if (rc != AG2V_OK) return rc;
+    }
+    return params ? run_params(a, a.N, sums, st) : AG2V_OK;
+}
+template <class E, int ACT>
+static int run_act(const GnArgs& a, const GnPlan& r, bool backward, float* ws, hipStream_t st) {
+    const bool past = past_caches<E>(a);
+    if (backward) return run_bwd<E, ACT>(a, r, past, ws, st);
+    for (int n0 = 0; n0 < a.N; n0 += r.per) {
+        const int rc = run_fwd<E, ACT>(samples_of<E>(a, n0, r.per), r, past, ws, st);
+        if (rc != AG2V_OK) return rc;
     }
     return AG2V_OK;
 }
 template <class E>
 static int run_elem(const GnArgs& a, const GnPlan& r, int act, bool backward, float* ws, hipStream_t st) {
-    if (act == ACT_SILU) return backward ? run_bwd<E, ACT_SILU>(a, r, ws, st) : run_fwd<E, ACT_SILU>(a, r, ws, st);
-    if (act == ACT_LRELU) return backward ? run_bwd<E, ACT_LRELU>(a, r, ws, st) : run_fwd<E, ACT_LRELU>(a, r, ws, st);
-    return backward ? run_bwd<E, ACT_NONE>(a, r, ws, st) : run_fwd<E, ACT_NONE>(a, r, ws, st);
+    if (act == ACT_SILU) return run_act<E, ACT_SILU>(a, r, backward, ws, st);
+    if (act == ACT_LRELU) return run_act<E, ACT_LRELU>(a, r, backward, ws, st);
+    return run_act<E, ACT_NONE>(a, r, backward, ws, st);
 }
 static int run_any(const GnArgs& a, int dtype, int act, bool backward, float* ws, size_t ws_floats, hipStream_t st) {
     const GnPlan r = plan_of(dtype, a.N, a.S, a.C, a.G, backward);
     if ((r.words && !ws) || ws_floats < (size_t)r.words || ((uintptr_t)ws & 15)) return AG2V_EINVAL;
-    if (!r.slab && ((long long)a.N * r.p.P * r.p.tiles >= (1LL << 24) || (long long)a.N * a.G * r.chunks >= (1LL << 24))) return AG2V_EINVAL;
     if (dtype == AG2V_F32) return run_elem<ElemF32>(a, r, act, backward, ws, st);
     return dtype == AG2V_BF16 ? run_elem<ElemBF16>(a, r, act, backward, ws, st) : run_elem<ElemF16>(a, r, act, backward, ws, st);
 }
