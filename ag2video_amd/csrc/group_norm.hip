@@ -777,41 +777,56 @@ __global__ __launch_bounds__(256) void gn_bwd_coef_kernel(int groups, int chunks
     if ((threadIdx.x & 63) == 0) coef[id] = make_float2(t1, t2);
 }
 
-// dw, db: 32 channels a workgroup at a time, 8 lanes a channel share its `rows` partial sums.
-__device__ __forceinline__ void params_of(const GnArgs& a, int blk, int nblk, int rows, const float2* ab) {
-    __shared__ float2 sh[256];
-    const int cl = threadIdx.x & 31, slot = threadIdx.x >> 5;
-    for (int c0 = blk * 32; c0 < a.C; c0 += nblk * 32) {
+// dw, db: 2^lcp channels a workgroup at a time, 256 >> lcp lanes a channel share its `rows` partial sums, eight in flight.  In fp64: each row is the
+// sum of a sample or of a walker's samples, and there may be a million of them.
+__device__ __forceinline__ void params_of(const GnArgs& a, int blk, int nblk, int lcp, int rows, const float2* ab) {
+    __shared__ double2 sh[256];
+    const int cl = threadIdx.x & ((1 << lcp) - 1), slot = threadIdx.x >> lcp, slots = 256 >> lcp;
+    for (int c0 = blk << lcp; c0 < a.C; c0 += nblk << lcp) {
         const int c = c0 + cl;
-        float2 v = make_float2(0.f, 0.f);
+        double vx = 0.0, vy = 0.0;
         if (c < a.C)
-            for (int r = slot; r < rows; r += 8) {
-                const float2 o = ab[(long long)r * a.C + c];
-                v.x += o.x;
-                v.y += o.y;
+            for (int r0 = slot; r0 < rows; r0 += 8 * slots) {
+                float2 o[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const long long r = r0 + (long long)u * slots;
+                    o[u] = r < rows ? ab[r * a.C + c] : make_float2(0.f, 0.f);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    vx += o[u].x;
+                    vy += o[u].y;
+                }
             }
-        sh[threadIdx.x] = v;
-        __syncthreads();
+        sh[threadIdx.x] = make_double2(vx, vy);
+        for (int o = slots >> 1; o > 0; o >>= 1) {
+            __syncthreads();
+            if (slot < o) {
+                const double2 q = sh[threadIdx.x + (o << lcp)];
+                vx += q.x;
+                vy += q.y;
+                sh[threadIdx.x] = make_double2(vx, vy);
+            }
+        }
         if (slot == 0 && c < a.C) {
-            for (int q = 1; q < 8; ++q) {
-                v.x += sh[q * 32 + cl].x;
-                v.y += sh[q * 32 + cl].y;
-            }
-            if (a.dw) store_any(a.dw, a.ptype, c, v.y);
-            if (a.db) store_any(a.db, a.ptype, c, v.x);
+            if (a.dw) store_any(a.dw, a.ptype, c, (float)vy);
+            if (a.db) store_any(a.db, a.ptype, c, (float)vx);
         }
         __syncthreads();
     }
 }
-__global__ __launch_bounds__(256) void gn_params_kernel(GnArgs a, int rows, const float2* ab) { params_of(a, blockIdx.x, gridDim.x, rows, ab); }
+__global__ __launch_bounds__(256) void gn_params_kernel(GnArgs a, int lcp, int rows, const float2* ab) {
+    params_of(a, blockIdx.x, gridDim.x, lcp, rows, ab);
+}
 
 // dx; the first `pblocks` workgroups sum the parameters' gradients instead.  NT: 1 stores past the caches, 2 loads too.  403 MB (4 x 65536 x 256
 // bf16) in 66 us, 6.1 TB/s: memory.
 template <class E, int ACT, int NT>
-__global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef, int pblocks, const float2* ab) {
+__global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, const float2* coef, int pblocks, int lcp, const float2* ab) {
     constexpr int V = E::V, U = 4;
     if ((int)blockIdx.x < pblocks) {
-        params_of(a, blockIdx.x, pblocks, a.N, ab);
+        params_of(a, blockIdx.x, pblocks, lcp, a.N, ab);
         return;
     }
     const GnWhere i = where_of<V>(a, p, blockIdx.x - pblocks);
@@ -936,7 +951,9 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
         if (per < N) r.per = (int)per;
     } else {                             // (any number of samples in one launch)
         long long wb = ((long long)N + subs - 1) / subs;
-        const long long cap = 2048 / r.s.nsets < 1 ? 1 : 2048 / r.s.nsets;
+        // at most 2048 workgroups, but no walker over 256 samples: it adds them up in fp32
+        long long cap = 2048 / r.s.nsets < 1 ? 1 : 2048 / r.s.nsets;
+        if (cap * subs * 256 < N) cap = ((long long)N + 256 * subs - 1) / (256 * subs);
         if (wb > cap) wb = cap;
         r.walkers = (int)wb * subs;
         r.words = 2LL * r.walkers * C;
@@ -1062,9 +1079,19 @@ static int run_fwd(const GnArgs& a, const GnPlan& r, bool past, float* ws, hipSt
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
+// Workgroups that sum the parameters' gradients, and log2 of the channels each takes at a time: 32, fewer where a channel's lanes would have over 64
+// rows each and few channels leave most of the chip without work (8192 x 16 x 16 fp32 in one group, 8192 rows: 61 us a backward pass, 257 with 32
+// channels a workgroup and one load in flight).
+static int param_blocks(int C, int rows, int& lcp) {
+    lcp = 5;
+    while (lcp > 0 && rows > 64 * (256 >> lcp) && C >> lcp < 64) --lcp;
+    const int blocks = ceil_div(C, 1 << lcp);
+    return blocks < GN_PARAM_BLOCKS ? blocks : GN_PARAM_BLOCKS;
+}
 static int run_params(const GnArgs& a, int rows, const float2* ab, hipStream_t st) {
-    const int blocks = ceil_div(a.C, 32);
-    hipLaunchKernelGGL(gn_params_kernel, dim3(blocks < GN_PARAM_BLOCKS ? blocks : GN_PARAM_BLOCKS), dim3(256), 0, st, a, rows, ab);
+    int lcp;
+    const int blocks = param_blocks(a.C, rows, lcp);
+    hipLaunchKernelGGL(gn_params_kernel, dim3(blocks), dim3(256), 0, st, a, lcp, rows, ab);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }
@@ -1083,14 +1110,15 @@ static int run_bwd_parts(const GnArgs& a, const GnPlan& r, bool past, bool param
         AG2V_CHECK_LAUNCH();
     }
     if (!a.y) return params ? run_params(a, a.N, sums, st) : AG2V_OK;
-    const int all = params ? ceil_div(a.C, 32) : 0, pblocks = all < GN_PARAM_BLOCKS ? all : GN_PARAM_BLOCKS;
+    int lcp = 0;
+    const int pblocks = params ? param_blocks(a.C, a.N, lcp) : 0;
     const dim3 grid(blocks + pblocks);
     if (past && r.p.tiles == 1)      // (x and dy together pass the bound of loads; the lines of a tiled row are read twice)
-        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 2>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 2>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, lcp, sums);
     else if (past)
-        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 1>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 1>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, lcp, sums);
     else
-        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 0>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, sums);
+        hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, 0>), grid, dim3(256), 0, st, a, r.p, coef, pblocks, lcp, sums);
     AG2V_CHECK_LAUNCH();
     return AG2V_OK;
 }

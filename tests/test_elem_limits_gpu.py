@@ -84,3 +84,27 @@ def test_very_wide_rows(n, V, D, dtype, device):
     for v in range(V):
         rows = dout[idx == v]
         assert torch.equal(got[v], rows.sum(0, dtype=torch.float32).mul(2).to(dtype) if rows.shape[0] else torch.zeros_like(got[v]))
+
+
+# One launch, whose workgroups walk many samples each, and parts, whose samples are added up at the end.
+@pytest.mark.parametrize("N,S,C", [(1 << 23, 16, 1), (1 << 18, 1100, 1), (1 << 20, 16, 12), (70000, 1500, 3)], ids=str)
+def test_parameter_gradients_of_very_many_samples(N, S, C, device):
+    """dbias where every term is the same number, whose last bits a long fp32 sum would drop one by one, and dweight.
+
+    No fp32 sum is deeper than a walker's 256 samples of at most two rows each and, before and behind it, the joins of a workgroup (14 levels)."""
+    from ag2video_amd import ops
+    c = (13107 + 63 / 128) / 2 ** 17                            # 21 bits
+    x = _normal(device, 1, N, S, C, dtype=torch.float32)
+    dy = torch.full((), c, device=device).expand(N, S, C)
+    p = [torch.full((C,), v, device=device, requires_grad=True) for v in (1.0, 0.0)]
+    dw, db = torch.autograd.grad(ops.group_norm_act(x, C, *p, act='none'), p, dy)
+    total = float(N) * S * c
+    depth = 256 + 2 + 14 + 1
+    assert ((db.double() - total).abs() <= depth * R.U * total).all(), ((db.double() - total) / total / R.U).tolist()
+    # dweight = c * sum of h, which is 0 but for rounding: that of the mean (DEPTH additions) in each h, and of the sums
+    mags = torch.zeros(C, device=device, dtype=torch.float64)
+    for part in x.split(1 << 18):
+        d = part.double()
+        d -= d.mean(1, keepdim=True)
+        mags += (d.abs() * ((d * d).mean(1, keepdim=True) + 1e-5) ** -0.5).sum((0, 1))
+    assert (dw.double().abs() <= c * (depth + 3 * R.DEPTH) * R.U * mags).all()
