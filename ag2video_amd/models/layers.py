@@ -20,6 +20,8 @@ class Embedding(nn.Embedding):
     """``scale`` (a number), ``padding_idx`` or a 16-bit table: ops.embedding_scaled (gradient by sorted tokens: for large vocabularies and
     long inputs).  Neither, in fp32: ops.embedding, as every table of the models here."""
 
+    scale = None        # (of modules that were pickled whole before there was one)
+
     def __init__(self, *args, scale=None, **kwargs):
         super().__init__(*args, **kwargs)
         self.scale = scale
