@@ -109,3 +109,24 @@ def test_gradients_far_from_zero(shape, G, act, device):
     ref = rstd * (t - s1 - h * s2)
     bound = rstd * (e_t + e_s1 + h.abs() * e_s2 + s2.abs() * e_h + 4 * R.U * (t.abs() + s1.abs() + (h * s2).abs())) + ref.abs() * (r_rstd + 2 * R.U)
     R.check('dx', dx.view(v.shape), ref, bound + R.U * (ref.abs() + bound))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize("shape,G", [((131, 64, 1024), 32), ((70, 64, 2048), 64), ((8199, 16, 16), 1), ((9001, 40, 16), 16), ((8201, 20, 12), 4), ((60, 200, 600), 200),
+                                     ((2100, 10, 90), 6), ((3001, 9, 72), 9)], ids=str)
+def test_batches_of_more_samples_than_workgroups(shape, G, dtype, device):
+    """The one-launch backward pass walks several samples a workgroup where a batch has more of them than 2048 workgroups: several rounds, the last one
+    not full, of one sample a workgroup and of four, of groups of whole vectors and of others."""
+    from ag2video_amd import ops
+    C = shape[-1]
+    x, dy = _randn(*shape, seed=1, dtype=dtype), _randn(*shape, seed=2, dtype=dtype)
+    w, b = 1 + 0.2 * _randn(C, seed=3), _randn(C, seed=4)
+    ref = R.group_norm(x, G, w, b, 1e-5, 'silu', 0.2, dy)
+    for name, got in zip(('y', 'dx', 'dweight', 'dbias'), _norm_all(device, x, G, w, b, dy, 'silu')):
+        R.check(name, got, *ref[name])
+    leaf = x.to(device).requires_grad_(True)
+    (dx,) = torch.autograd.grad(ops.group_norm_act(leaf, G, w.to(device), b.to(device)), leaf, dy.to(device))
+    for n in (0, shape[0] // 2, shape[0] - 1):
+        one = x[n:n + 1].to(device).requires_grad_(True)
+        (d1,) = torch.autograd.grad(ops.group_norm_act(one, G, w.to(device), b.to(device)), one, dy[n:n + 1].to(device))
+        assert torch.equal(d1[0], dx[n])
