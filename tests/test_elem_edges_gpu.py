@@ -130,3 +130,68 @@ def test_batches_of_more_samples_than_workgroups(shape, G, dtype, device):
         one = x[n:n + 1].to(device).requires_grad_(True)
         (d1,) = torch.autograd.grad(ops.group_norm_act(one, G, w.to(device), b.to(device)), one, dy[n:n + 1].to(device))
         assert torch.equal(d1[0], dx[n])
+
+
+@pytest.mark.parametrize("view", [lambda t: t, lambda t: t[..., 3:]], ids=['whole', 'slice'])
+def test_group_norm_backward_past_32_bit_offsets(view, device):
+    """x, dy and dx of more than 2^31 elements, all different: each sample as it is alone."""
+    from ag2video_amd import ops
+    N, S, C = 3, 1 << 20, 720
+    x, dy = (torch.empty(N, S, C, device=device, dtype=torch.bfloat16) for _ in range(2))
+    for n in range(N):
+        x[n].normal_(generator=torch.Generator(device=device).manual_seed(n))
+        dy[n].normal_(generator=torch.Generator(device=device).manual_seed(10 + n))
+    x, dy = view(x), view(dy)
+    C = x.shape[-1]
+    G = 3
+    w = [_randn(C, seed=1).to(device).requires_grad_(True), _randn(C, seed=2).to(device).requires_grad_(True)]
+    leaf = x.detach().requires_grad_(True)
+    dx, dw, db = torch.autograd.grad(ops.group_norm_act(leaf, G, *w), [leaf] + w, dy)
+    sums, mags = torch.zeros(2, C, device=device, dtype=torch.float64), torch.zeros(2, C, device=device, dtype=torch.float64)
+    for n in range(N):
+        one = x.detach()[n:n + 1].clone().requires_grad_(True)
+        d1, *p1 = torch.autograd.grad(ops.group_norm_act(one, G, *w), [one] + w, dy[n:n + 1].clone())
+        assert torch.equal(d1[0], dx[n])
+        p1 = torch.stack(p1).double()
+        sums += p1
+        mags += p1.abs()
+    # one rounding of each sample's own, and one of the sum
+    assert ((torch.stack((dw, db)).double() - sums).abs() <= R.U * (mags + sums.abs())).all()
+    del x, dy, dx, leaf, one, d1
+    torch.cuda.empty_cache()
+
+
+# The ways of the gradient: one launch, tiles, ranks, a radix sort; rows far apart where there are few of them.
+@pytest.mark.parametrize("n,V,D,apart", [(2000, 4, 64, 1 << 21), ((1 << 20) - 5, 27, 2100, 2100), (8000, 3000, 33, 1 << 19), ((1 << 25) + 77, 50, 72, 72),
+                                         (300000, 3000, 40, 1 << 13)], ids=['one launch', 'tiles', 'ranks', 'radix, few words', 'radix'])
+def test_embedding_gradient_rows_past_32_bit_offsets(n, V, D, apart, device):
+    """A dense gradient of more than 2^31 elements, zero but for rows on both sides of that offset and the last ones.  Whole numbers."""
+    from ag2video_amd import ops
+    wide = torch.zeros(n, apart, device=device, dtype=torch.bfloat16)
+    idx = (torch.arange(n, device=device) * 7 + 3) % V
+    border = (1 << 31) // apart
+    rows = torch.tensor(sorted({0, 1, border - 1, border, border + 1, border + n // 100, n - 2, n - 1}), device=device)
+    assert border + n // 100 < n
+    values = torch.randint(-8, 9, (rows.numel(), D), generator=torch.Generator().manual_seed(1)).to(device)
+    wide[rows, :D] = values.bfloat16()
+    table = torch.zeros(V, D, device=device, dtype=torch.bfloat16, requires_grad=True)
+    (got,) = torch.autograd.grad(ops.embedding_scaled(idx, table, 2.0), table, wide[:, :D])
+    want = torch.zeros(V, D, device=device, dtype=torch.float64).index_add_(0, idx[rows], values.double()) * 2
+    assert want.any() and torch.equal(got.double(), want)
+    del wide
+    torch.cuda.empty_cache()
+
+
+def test_embedding_tokens_past_32_bit_offsets(device):
+    """Tokens 2^20 elements apart."""
+    from ag2video_amd import ops
+    n, V, D = 3000, 500, 12
+    far = torch.zeros(n, 1 << 20, device=device, dtype=torch.int32)
+    idx = torch.randint(V, (n,), generator=torch.Generator().manual_seed(1)).to(device)
+    far[:, 5] = idx.int()
+    table, dout = _randn(V, D, seed=2).to(device).requires_grad_(True), _randn(n, D, seed=3).to(device)
+    a, b = ops.embedding_scaled(far[:, 5], table), ops.embedding_scaled(idx, table)
+    assert torch.equal(a, b)
+    assert torch.equal(torch.autograd.grad(a, table, dout)[0], torch.autograd.grad(b, table, dout)[0])
+    del far
+    torch.cuda.empty_cache()
