@@ -4,7 +4,7 @@
 //     z = w h + b                y = act(z):  0 z,  1 z * sigmoid(z),  2 z > 0 ? z : slope * z
 //   backward, dz = dy act'(z), A[n,c] = sum_s dz, B[n,c] = sum_s dz h:
 //     db = sum_n A, dw = sum_n B, s1 = sum_{c in g} w A, s2 = sum_{c in g} w B, dx = rstd (w dz - (s1 + h s2) / M)
-// Every sum is in fp32; z and h are computed again in the backward pass from x and the two statistics of a group: h as written, because the
+// Sums are in fp32, the joins of a group's parts and of the parameters' rows in fp64; z and h are computed again in the backward pass from x and the two statistics of a group: h as written, because the
 // rounding of mean * rstd in x * rstd - mean * rstd would be one of |mean| rstd 2^-24 in h, more than all else where the mean is far from zero.
 //
 // Memory bounds all of it: forward x is read and y written, backward x and dy are read and dx written.  A (sample, set of groups) that fits
@@ -136,7 +136,7 @@ static int log2_up(long long v) {
 // it, then the result.  blockDim / T slabs a workgroup.  ONE: a thread's vector touches one group (Cg a multiple of the vector, or kg = 1);
 // otherwise sums and statistics are per channel.
 // 6.0 us for 1 x 64 x 1024 bf16 and for 8 x 64 x 1024 fp32, of which an empty kernel's launch is 2 and the chain load - sum - squares - store
-// the rest.  20 us for 8 x 4096 x 256 fp16 in 32 groups, whose rows are one vector each: 1.6 TB/s, bound by 16-byte pieces of cache lines.
+// the rest.  20 us for 8 x 4096 x 256 fp16 in 32 groups, two of them a slab: 1.6 TB/s, bound by its 128 workgroups, which leave half of the CUs without work.
 struct GnSlab {
     int T, kg, nsets;                  // threads, groups, sets of groups a sample
     int lc, rows, slots, wg, llg;      // log2 of vectors a row, rows at a time, LDS slots, columns a group there, log2 of lanes a group
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
 // Backward on slabs: x and dy of a slab in registers.  A workgroup keeps its set of groups and walks samples, `walkers` apart, so that the
 // parameters' gradients leave it once: ab[walker][C] = (sum dz, sum dz h) over its samples.  Without ONE the statistics are per channel and
 // take up to 256 registers a thread; with ONE the bound of 1024 threads keeps them to 128, so that two workgroups of 512 fit a CU (64 x 1024 x 256
-// bf16: 58 us with 128 and 82 with 136).  7.3 us for 8 x 64 x 1024 fp32, bound by the chain of loads and joins.
+// bf16: 58 us with 128 and 82 with 136).  7.2 us for 8 x 64 x 1024 fp32, bound by the chain of loads and joins.
 template <class E, int ACT, int U, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a, GnSlab p, int walkers, float2* ab) {
     extern __shared__ float shm[];
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(GnArgs a, GnParts p, floa
     }
 }
 
-// A wave per (sample, group): the mean of its parts' means, then the squares about it, in fp64.  4.7 us for 512 groups of 256 parts, two
+// A wave per (sample, group): the mean of its parts' means, then the squares about it, in fp64.  4.8 us for 512 groups of 256 parts, two
 // rounds of loads and shuffles.
 template <int V>
 __global__ __launch_bounds__(256) void gn_stats_join_kernel(GnArgs a, GnParts p, const float4* part) {
@@ -645,7 +645,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(GnArgs a, GnParts p, cons
     }
 }
 
-// part[n][q][c] = (sum dz, sum dz h) over the part's positions.  268 MB (4 x 65536 x 256 bf16) in 51 us, 5.3 TB/s: memory.
+// part[n][q][c] = (sum dz, sum dz h) over the part's positions.  268 MB (4 x 65536 x 256 bf16) in 48 us, 5.6 TB/s: memory.
 template <class E, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, float2* part) {
     constexpr int V = E::V, U = 4;
@@ -706,7 +706,7 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
 }
 
 // `chunks` workgroups per (sample, group): the parts of its channels, in order; ab[n][c], and the (s1 / M, s2 / M) of a workgroup's channels to
-// coef[n][g][chunk].  5.6 us for 128 groups of 8 channels in 512 parts.
+// coef[n][g][chunk].  5.2 us for 128 groups of 8 channels in 512 parts.
 __global__ __launch_bounds__(256) void gn_bwd_join_kernel(GnArgs a, int P, int lcw, int chunks, const float2* part, float2* ab, float2* coef) {
     __shared__ float2 sh[256];
     const int ng = blockIdx.x / chunks, n = ng / a.G, g = ng - n * a.G;
@@ -882,8 +882,8 @@ struct GnPlan {
     int lcw, chunks;                 // backward: log2 of the channels, and workgroups a group, that join the parts
     long long words, ab, coef, chunk;       // workspace in floats; offsets of ab[][C], coef[N][G] and the chunks' in it
 };
-// Vectors of a slab at most.  Forward, 8192 (8 x 4096 x 256 fp16: 17 us, in parts 20; 64 x 1961 x 90 fp32 32 and 35).  Backward, where x and dy
-// are held, 1024: the 2000 vectors of 64 x 2000 x 64 fp16 in 8 groups took 55 us a training pass, 44 in parts, and 24 and 19.5 for one sample.
+// Vectors of a slab at most.  Forward, 8192: 4096 x 256 fp16 in 32 groups, replayed, take 13.6 us (one sample), 19.4 (8) and 92 (64), in parts of the same
+// build 15.7, 21.4 and 82; 1961 x 90 fp32 in 6 groups 10.3, 11.3 and 32.5, in parts 10.9, 12.4 and 33.6.  Backward, where x and dy are held, 1024: the 2000 vectors of 64 x 2000 x 64 fp16 in 8 groups took 55 us a training pass, 44 in parts, and 24 and 19.5 for one sample.
 #define GN_SLAB_FWD 8192
 #define GN_SLAB_BWD 1024
 #define GN_JOIN_SPLIT 8192
@@ -908,7 +908,7 @@ static bool plan_slab(GnPlan& r, int V, int N, int S, int C, int G, bool backwar
     const int lc = lcols(kg);
     // Narrow rows of a larger map: every cache line would be fetched by many slabs, in pieces (13 x 1085 x 1560 fp16 in 195 groups, one vector a
     // row: 147 us a training pass, 72 us in parts; 11 x 4181 x 45 fp32 in 15 groups, 12 bytes a row: 49 and 37 us).  Forward, rows of whole
-    // vectors are no slower here (8 x 4096 x 256 fp16 in 32 groups: 20.4 us, in parts 22) and take one launch.
+    // vectors take one launch and are no slower up to 8 samples (figures at GN_SLAB_FWD).
     if (kg < G && (long long)kg * Cg < V && S > 2048) return false;
     const long long held = (long long)S << lc;
     if (!small && kg < G && !backward && (long long)kg * Cg < 2 * V && Cg % V) return false;
