@@ -206,9 +206,10 @@ struct EmbeddingScaled : torch::autograd::Function<EmbeddingScaled> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         first_derivative_only("embedding_scaled");
+        const Tensor idx = ctx->get_saved_variables()[0];      // (above the guard: a checkpoint runs its forward pass again in here)
         at::AutoDispatchBelowADInplaceOrView below;
-        Tensor dtable = embedding_backward_call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["V"].toInt(),
-                                                ctx->saved_data["scale"].toDouble(), ctx->saved_data["pad"].toInt());
+        Tensor dtable = embedding_backward_call(grads[0], idx, ctx->saved_data["V"].toInt(), ctx->saved_data["scale"].toDouble(),
+                                                ctx->saved_data["pad"].toInt());
         return {Tensor(), dtable, Tensor(), Tensor()};
     }
 };

@@ -4,8 +4,9 @@
 //     z = w h + b                y = act(z):  0 z,  1 z * sigmoid(z),  2 z > 0 ? z : slope * z
 //   backward, dz = dy act'(z), A[n,c] = sum_s dz, B[n,c] = sum_s dz h:
 //     db = sum_n A, dw = sum_n B, s1 = sum_{c in g} w A, s2 = sum_{c in g} w B, dx = rstd (w dz - (s1 + h s2) / M)
-// Sums are in fp32, the joins of a group's parts and of the parameters' rows in fp64; z and h are computed again in the backward pass from x and the two statistics of a group: h as written, because the
-// rounding of mean * rstd in x * rstd - mean * rstd would be one of |mean| rstd 2^-24 in h, more than all else where the mean is far from zero.
+// Sums are in fp32, the joins of a group's parts and of the parameters' rows in fp64.  z and h are computed again in the backward pass from x and the
+// two statistics of a group: h as written, because the rounding of mean * rstd in x * rstd - mean * rstd would be one of |mean| rstd 2^-24 in h, more
+// than all else where the mean is far from zero.
 //
 // Memory bounds all of it: forward x is read and y written, backward x and dy are read and dx written.  A (sample, set of groups) that fits
 // the registers of a workgroup is read once, in one launch (gn_slab_*).  A larger one is read twice: parts of a sample's positions give
@@ -883,7 +884,8 @@ struct GnPlan {
     long long words, ab, coef, chunk;       // workspace in floats; offsets of ab[][C], coef[N][G] and the chunks' in it
 };
 // Vectors of a slab at most.  Forward, 8192: 4096 x 256 fp16 in 32 groups, replayed, take 13.6 us (one sample), 19.4 (8) and 92 (64), in parts of the same
-// build 15.7, 21.4 and 82; 1961 x 90 fp32 in 6 groups 10.3, 11.3 and 32.5, in parts 10.9, 12.4 and 33.6.  Backward, where x and dy are held, 1024: the 2000 vectors of 64 x 2000 x 64 fp16 in 8 groups took 55 us a training pass, 44 in parts, and 24 and 19.5 for one sample.
+// build 15.7, 21.4 and 82; 1961 x 90 fp32 in 6 groups 10.3, 11.3 and 32.5, in parts 10.9, 12.4 and 33.6.  Backward, where x and dy are held, 1024:
+// the 2000 vectors of 64 x 2000 x 64 fp16 in 8 groups took 55 us a training pass, 44 in parts, and 24 and 19.5 for one sample.
 #define GN_SLAB_FWD 8192
 #define GN_SLAB_BWD 1024
 #define GN_JOIN_SPLIT 8192

@@ -195,3 +195,26 @@ def test_embedding_tokens_past_32_bit_offsets(device):
     assert torch.equal(torch.autograd.grad(a, table, dout)[0], torch.autograd.grad(b, table, dout)[0])
     del far
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape,G", [((3, 50, 24), 3), ((2, 6000, 36), 4), ((1, 4, 8192), 1)], ids=str)
+def test_gradients_of_some_inputs_alone(shape, G, device):
+    """x, weight and bias with a gradient or without, and absent: the same bits as all of them together."""
+    from ag2video_amd import ops
+    C = shape[-1]
+    x, dy = _randn(*shape, seed=1).to(device), _randn(*shape, seed=2).to(device)
+    w, b = (1 + 0.2 * _randn(C, seed=3)).to(device), _randn(C, seed=4).to(device)
+    for have in ((True, True), (True, False), (False, True)):
+        tensors = [x] + [t if h else None for t, h in zip((w, b), have)]
+        leaves = [None if t is None else t.clone().requires_grad_(True) for t in tensors]
+        y = ops.group_norm_act(leaves[0], G, *leaves[1:])
+        full = dict(zip([k for k in range(3) if leaves[k] is not None], torch.autograd.grad(y, [t for t in leaves if t is not None], dy)))
+        for mask in range(1, 8):
+            want = [k for k in range(3) if mask >> k & 1 and tensors[k] is not None]
+            if not want:
+                continue
+            some = [None if t is None else t.clone().requires_grad_(k in want) for k, t in enumerate(tensors)]
+            y1 = ops.group_norm_act(some[0], G, *some[1:])
+            assert torch.equal(y1, y)
+            for k, g in zip(want, torch.autograd.grad(y1, [some[k] for k in want], dy)):
+                assert torch.equal(g, full[k]), (have, want, k)

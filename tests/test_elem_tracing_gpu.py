@@ -200,3 +200,30 @@ def test_recorded_operators_refuse_what_the_functions_refuse(device):
             with pytest.raises((RuntimeError, NotImplementedError)):
                 fn(*args)
                 pytest.fail('%s %d was not refused' % (fn, k))
+
+
+@pytest.mark.parametrize("fn", CALLS)
+def test_modes_of_torch(fn, device):
+    """inference_mode, autocast, checkpoints of either kind, and a saved trace: the plain call's bits."""
+    import io
+    from torch.utils.checkpoint import checkpoint
+    plain = _inputs(fn, 1, True)
+    want = fn(*plain)
+    grads = _grads(want, plain)
+    with torch.inference_mode():
+        assert torch.equal(fn(*_inputs(fn, 1)), want)
+    with torch.autocast('cuda', torch.bfloat16):
+        assert torch.equal(fn(*_inputs(fn, 1)), want)
+    for reentrant in (False, True):
+        again = _inputs(fn, 1, True)
+        y = checkpoint(fn, *again, use_reentrant=reentrant)
+        assert torch.equal(y, want)
+        leaves = [t for t in again if t.requires_grad]
+        y.backward(_randn(*y.shape, seed=9, dtype=y.dtype))
+        assert all(torch.equal(t.grad, g) for t, g in zip(leaves, grads))
+    with warnings.catch_warnings():
+        warnings.simplefilter('ignore')
+        buffer = io.BytesIO()
+        torch.jit.save(torch.jit.trace(fn, _inputs(fn, 0)), buffer)
+        buffer.seek(0)
+        assert torch.equal(torch.jit.load(buffer)(*_inputs(fn, 1)), want)
