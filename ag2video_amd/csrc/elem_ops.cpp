@@ -111,7 +111,10 @@ void first_derivative_only(const char* name) {
 void reverse_mode_only(const char* name, std::initializer_list<const Tensor*> inputs) {
     for (const Tensor* t : inputs) TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative");
 }
-Tensor given(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
+const Tensor& given(const std::optional<Tensor>& t) {
+    static const Tensor none;
+    return t ? *t : none;
+}
 std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 bool wants_grad(std::initializer_list<const Tensor*> inputs) {
     if (!at::GradMode::is_enabled()) return false;
@@ -233,6 +236,8 @@ int param_type(const Tensor& weight, const Tensor& bias) {
 int64_t positions(const Tensor& x) { return x.numel() ? x.numel() / x.size(0) / x.size(-1) : 0; }
 Tensor dense_like(const Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous)); }
 
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
 void norm_check(const Tensor& x, int64_t groups, const Tensor& weight, const Tensor& bias, double eps, int64_t act, double slope) {
     const char* name = "group_norm_act";
     TORCH_CHECK(elem_of(x.scalar_type()) >= 0, name, ": expected float32, bfloat16 or float16, got ", x.scalar_type());
@@ -257,18 +262,16 @@ typedef std::optional<Tensor> Param;
 std::tuple<Tensor, Tensor> norm_results(const Tensor& x, int64_t groups) {
     return {dense_like(x), at::empty({2, x.size(0), groups}, x.options().requires_grad(false).dtype(at::kFloat))};
 }
-std::tuple<Tensor, Tensor> norm_meta(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, int64_t act, double slope) {
+std::tuple<Tensor, Tensor> norm_stats_meta(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, int64_t act, double slope) {
     norm_check(x, groups, given(weight), given(bias), eps, act, slope);
     return norm_results(x, groups);
 }
 // y, and mean and 1 / std of every (sample, group)
-std::tuple<Tensor, Tensor> norm_device(const Tensor& x, int64_t groups, const Param& weight_, const Param& bias_, double eps, int64_t act, double slope) {
-    Tensor weight = given(weight_), bias = given(bias_);
-    norm_check(x, groups, weight, bias, eps, act, slope);
+std::tuple<Tensor, Tensor> norm_stats_device(const Tensor& x, int64_t groups, const Param& weight_, const Param& bias_, double eps, int64_t act, double slope) {
+    norm_check(x, groups, given(weight_), given(bias_), eps, act, slope);
     auto [y, stats] = norm_results(x, groups);
     if (x.numel() == 0) return {y, stats};
-    if (weight.defined()) weight = weight.contiguous();
-    if (bias.defined()) bias = bias.contiguous();
+    const Tensor weight = dense(given(weight_)), bias = dense(given(bias_));
     const int64_t N = x.size(0), C = x.size(-1), S = positions(x);
     const auto [rows, xs, xr] = channel_rows(x);
     OnDevice on(x);
@@ -281,6 +284,12 @@ std::tuple<Tensor, Tensor> norm_device(const Tensor& x, int64_t groups, const Pa
                                                 static_cast<float*>(ptr(ws)), floats, on.stream));
     return {y, stats};
 }
+Tensor norm_meta(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, int64_t act, double slope) {
+    return std::get<0>(norm_stats_meta(x, groups, weight, bias, eps, act, slope));
+}
+Tensor norm_device(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, int64_t act, double slope) {
+    return std::get<0>(norm_stats_device(x, groups, weight, bias, eps, act, slope));
+}
 void norm_backward_check(const Tensor& dy, const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& stats, int64_t act, double slope) {
     const char* name = "group_norm_act_backward";
     TORCH_CHECK(x.dim() >= 2 && stats.dim() == 3 && stats.size(0) == 2 && stats.size(1) == x.size(0) && stats.scalar_type() == at::kFloat &&
@@ -292,7 +301,7 @@ void norm_backward_check(const Tensor& dy, const Tensor& x, const Tensor& weight
 typedef std::tuple<Tensor, Tensor, Tensor> Grads;      // of x, weight and bias; undefined where not wanted
 Grads norm_backward_meta(const Tensor& dy, const Tensor& x, const Param& weight_, const Param& bias_, const Tensor& stats, int64_t act, double slope,
                          std::array<bool, 3> wanted) {
-    const Tensor weight = given(weight_), bias = given(bias_);
+    const Tensor &weight = given(weight_), &bias = given(bias_);
     norm_backward_check(dy, x, weight, bias, stats, act, slope);
     return {wanted[0] ? dense_like(x) : Tensor(), wanted[1] && weight.defined() ? dense_like(weight) : Tensor(),
             wanted[2] && bias.defined() ? dense_like(bias) : Tensor()};
@@ -305,9 +314,7 @@ Grads norm_backward_device(const Tensor& dy, const Tensor& x, const Param& weigh
             if (t->defined()) t->zero_();
         return {dx, dw, db};
     }
-    Tensor weight = given(weight_), bias = given(bias_);
-    if (weight.defined()) weight = weight.contiguous();
-    if (bias.defined()) bias = bias.contiguous();
+    const Tensor weight = dense(given(weight_)), bias = dense(given(bias_));
     const int64_t N = x.size(0), C = x.size(-1), S = positions(x), groups = stats.size(2);
     const auto [xrows, xs, xr] = channel_rows(x);
     const auto [drows, ds, dr] = channel_rows(dy);
@@ -321,8 +328,13 @@ Grads norm_backward_device(const Tensor& dy, const Tensor& x, const Param& weigh
                                                 int(groups), int(act), float(slope), static_cast<float*>(ptr(ws)), floats, on.stream));
     return {dx, dw, db};
 }
-std::tuple<Tensor, Tensor> norm_call(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, int64_t act, double slope) {
+Tensor norm_call(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, int64_t act, double slope) {
     static const auto op = op_of<decltype(norm_device)>("ag2v::group_norm_act");
+    return op.call(x, groups, weight, bias, eps, act, slope);
+}
+std::tuple<Tensor, Tensor> norm_stats_call(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, int64_t act,
+                                           double slope) {
+    static const auto op = op_of<decltype(norm_stats_device)>("ag2v::group_norm_act_stats");
     return op.call(x, groups, weight, bias, eps, act, slope);
 }
 Grads norm_backward_call(const Tensor& dy, const Tensor& x, const Param& weight, const Param& bias, const Tensor& stats, int64_t act, double slope,
@@ -332,20 +344,17 @@ Grads norm_backward_call(const Tensor& dy, const Tensor& x, const Param& weight,
 }
 
 struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Param& weight, const Param& bias, int64_t groups, double eps, int64_t act,
-                                 double slope) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Param& weight, const Param& bias, int64_t groups, double eps, int64_t act,
+                          double slope) {
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [y, stats] = norm_call(x, groups, weight, bias, eps, act, slope);
+        auto [y, stats] = norm_stats_call(x, groups, weight, bias, eps, act, slope);
         ctx->save_for_backward({x, given(weight), given(bias), stats});
-        ctx->mark_non_differentiable({stats});
-        ctx->set_materialize_grads(false);          // (nothing is to be launched for the statistics)
         ctx->saved_data["act"] = act;
         ctx->saved_data["slope"] = slope;
-        return {y, stats};
+        return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         first_derivative_only("group_norm_act");
-        if (!grads[0].defined()) return variable_list(7);
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
         at::AutoDispatchBelowADInplaceOrView below;
@@ -357,29 +366,27 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
-std::tuple<Tensor, Tensor> norm_autograd(const Tensor& x, int64_t groups, const Param& weight_, const Param& bias_, double eps, int64_t act, double slope) {
-    const Tensor weight = given(weight_), bias = given(bias_);
-    reverse_mode_only("group_norm_act", {&x, &weight, &bias});
-    if (wants_grad({&x, &weight, &bias})) {
-        const variable_list r = GroupNormAct::apply(x, maybe(weight), maybe(bias), groups, eps, act, slope);
-        return {r[0], r[1]};
-    }
+Tensor norm_autograd(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, int64_t act, double slope) {
+    reverse_mode_only("group_norm_act", {&x, &given(weight), &given(bias)});
+    if (wants_grad({&x, &given(weight), &given(bias)})) return GroupNormAct::apply(x, weight, bias, groups, eps, act, slope);
     at::AutoDispatchBelowADInplaceOrView below;
-    return norm_call(x, groups, weight_, bias_, eps, act, slope);
+    return norm_call(x, groups, weight, bias, eps, act, slope);
 }
 
 Tensor group_norm_act(const Tensor& x, int64_t groups, const Param& weight, const Param& bias, double eps, const std::string& act, double slope) {
     elem_check("group_norm_act", x);
     const int64_t code = act == "silu" ? 1 : act == "lrelu" ? 2 : act == "none" ? 0 : -1;
     TORCH_CHECK(code >= 0, "group_norm_act: unknown activation '", act, "' (silu, lrelu, none)");
-    return std::get<0>(norm_call(x, groups, weight, bias, eps, code, slope));
+    return norm_call(x, groups, weight, bias, eps, code, slope);
 }
 }  // namespace
 
 TORCH_LIBRARY(ag2v, m) {
     m.def("embedding_scaled(Tensor idx, Tensor table, float scale, int padding_idx) -> Tensor");
     m.def("embedding_scaled_backward(Tensor dout, Tensor idx, int rows, float scale, int padding_idx) -> Tensor");
-    m.def("group_norm_act(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act, float slope) -> (Tensor, Tensor)");
+    m.def("group_norm_act(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act, float slope) -> Tensor");
+    // with the statistics, for the tape: no derivative of its own
+    m.def("group_norm_act_stats(Tensor x, int groups, Tensor? weight, Tensor? bias, float eps, int act, float slope) -> (Tensor, Tensor)");
     m.def("group_norm_act_backward(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor stats, int act, float slope, bool[3] wanted)"
           " -> (Tensor, Tensor, Tensor)");
 }
@@ -387,12 +394,14 @@ TORCH_LIBRARY_IMPL(ag2v, CUDA, m) {         // (the key of HIP devices)
     m.impl("embedding_scaled", &embedding_device);
     m.impl("embedding_scaled_backward", &embedding_backward_device);
     m.impl("group_norm_act", &norm_device);
+    m.impl("group_norm_act_stats", &norm_stats_device);
     m.impl("group_norm_act_backward", &norm_backward_device);
 }
 TORCH_LIBRARY_IMPL(ag2v, Meta, m) {
     m.impl("embedding_scaled", &embedding_meta);
     m.impl("embedding_scaled_backward", &embedding_backward_meta);
     m.impl("group_norm_act", &norm_meta);
+    m.impl("group_norm_act_stats", &norm_stats_meta);
     m.impl("group_norm_act_backward", &norm_backward_meta);
 }
 TORCH_LIBRARY_IMPL(ag2v, Autograd, m) {
