@@ -5,8 +5,8 @@
 //   backward, dz = dy act'(z), A[n,c] = sum_s dz, B[n,c] = sum_s dz h:
 //     db = sum_n A, dw = sum_n B, s1 = sum_{c in g} w A, s2 = sum_{c in g} w B, dx = rstd (w dz - (s1 + h s2) / M)
 // Sums are in fp32, the joins of a group's parts and of the parameters' rows in fp64.  z and h are computed again in the backward pass from x and the
-// two statistics of a group: h as written, because the rounding of mean * rstd in x * rstd - mean * rstd would be one of |mean| rstd 2^-24 in h, more
-// than all else where the mean is far from zero.
+// two statistics of a group, by way of x - mean as in the forward pass: the rounding of mean * rstd in x * rstd - mean * rstd would be one of
+// |mean| rstd 2^-24 in h, more than all else where the mean is far from zero.  B = rstd sum dz (x - mean).
 //
 // Memory bounds all of it: forward x is read and y written, backward x and dy are read and dx written.  A (sample, set of groups) that fits
 // the registers of a workgroup is read once, in one launch (gn_slab_*).  A larger one is read twice: parts of a sample's positions give
@@ -313,13 +313,14 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = (v[k] - mean[k % NG]) * rstd[k % NG], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                        const float e = v[k] - mean[k % NG], dz = act_bwd<ACT>(d[k], fmaf(e, w[k] * rstd[k % NG], b[k]), a.slope);
                         sA[k] += dz;
-                        sB[k] = fmaf(dz, h, sB[k]);
+                        sB[k] = fmaf(dz, e, sB[k]);
                     }
                 }
 #pragma unroll
             for (int k = 0; k < V; ++k) {
+                sB[k] *= rstd[k % NG];
                 A[k] += sA[k];
                 B[k] += sB[k];
                 if (k >= dup && at + k < W) {      // (w and b behind W are the next group's)
@@ -353,8 +354,8 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
             for (int u = 0; u < U; ++u) asm volatile("" : "+v"(rx[u]), "+v"(rd[u]));
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
-                g1[k] = stat[gi[k]] * inv;
-                g2[k] = stat[p.kg + gi[k]] * inv;
+                g1[k] = stat[gi[k]] * inv * rstd[k];
+                g2[k] = stat[p.kg + gi[k]] * inv * rstd[k];
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -365,8 +366,8 @@ __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a,
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = (v[k] - mean[k % NG]) * rstd[k % NG], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
-                        v[k] = rstd[k % NG] * (w[k] * dz - g1[k % NG] - h * g2[k % NG]);
+                        const float e = v[k] - mean[k % NG], wr = w[k] * rstd[k % NG], dz = act_bwd<ACT>(d[k], fmaf(e, wr, b[k]), a.slope);
+                        v[k] = fmaf(-(e * rstd[k % NG]), g2[k % NG], fmaf(dz, wr, -g1[k % NG]));
                     }
                     store_tail<E>(dx + (long long)r * a.C, dup, W, v);
                 }
@@ -659,6 +660,8 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
         load_params<E>(a.w, a.ptype, i.c, a.C, 1.f, w);
         load_params<E>(a.b, a.ptype, i.c, a.C, 0.f, b);
         load_stats<V>(a, i.n, i.c, mean, rstd);
+#pragma unroll
+        for (int k = 0; k < V; ++k) w[k] *= rstd[k];
         const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
         const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c;
         for (int r = i.lo + i.rs; r < i.hi; r += U * p.rows) {
@@ -677,12 +680,14 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(GnArgs a, GnParts p, f
                     E::unpack(rd[u], d);
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const float h = (v[k] - mean[k]) * rstd[k], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
+                        const float e = v[k] - mean[k], dz = act_bwd<ACT>(d[k], fmaf(e, w[k], b[k]), a.slope);
                         A[k] += dz;
-                        B[k] = fmaf(dz, h, B[k]);
+                        B[k] = fmaf(dz, e, B[k]);
                     }
                 }
         }
+#pragma unroll
+        for (int k = 0; k < V; ++k) B[k] *= rstd[k];
     }
     same_vector_sums(A, cols);
     same_vector_sums(B, cols);
@@ -837,6 +842,12 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
     load_params<E>(a.w, a.ptype, i.c, a.C, 1.f, w);
     load_params<E>(a.b, a.ptype, i.c, a.C, 0.f, b);
     load_stats<V>(a, i.n, i.c, mean, rstd, coef, cf);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        w[k] *= rstd[k];
+        cf[k].x *= rstd[k];
+        cf[k].y *= rstd[k];
+    }
     const typename E::T* x = (const typename E::T*)a.x + i.n * a.xs + i.c;
     const typename E::T* dy = (const typename E::T*)a.dy + i.n * a.ds + i.c;
     typename E::T* dx = (typename E::T*)a.y + (long long)i.n * a.S * a.C + i.c;
@@ -856,8 +867,8 @@ __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(GnArgs a, GnParts p, con
                 E::unpack(rd[u], d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    const float h = (v[k] - mean[k]) * rstd[k], dz = act_bwd<ACT>(d[k], fmaf(h, w[k], b[k]), a.slope);
-                    v[k] = rstd[k] * (w[k] * dz - cf[k].x - h * cf[k].y);
+                    const float e = v[k] - mean[k], dz = act_bwd<ACT>(d[k], fmaf(e, w[k], b[k]), a.slope);
+                    v[k] = fmaf(-(e * rstd[k]), cf[k].y, fmaf(dz, w[k], -cf[k].x));
                 }
                 store_tail<E, NT != 0>(dx + (long long)(r + u * p.rows) * a.C, i.dup, a.C, v);
             }
