@@ -256,7 +256,7 @@ __global__ __launch_bounds__(1024) void gn_slab_fwd_kernel(GnArgs a, GnSlab p) {
 // Backward on slabs: x and dy of a slab in registers.  A workgroup keeps its set of groups and walks samples, `walkers` apart, so that the
 // parameters' gradients leave it once: ab[walker][C] = (sum dz, sum dz h) over its samples.  Without ONE the statistics are per channel and
 // take up to 256 registers a thread; with ONE the bound of 1024 threads keeps them to 128, so that two workgroups of 512 fit a CU (64 x 1024 x 256
-// bf16: 58 us with 128 and 82 with 136).  7.2 us for 8 x 64 x 1024 fp32, bound by the chain of loads and joins.
+// bf16: 58 us with 128 and 82 with 136).  7 to 9 us for 8 x 64 x 1024 fp32 (medians of runs), bound by the chain of loads and joins.
 template <class E, int ACT, int U, bool ONE>
 __global__ __launch_bounds__(ONE ? 1024 : 512) void gn_slab_bwd_kernel(GnArgs a, GnSlab p, int walkers, float2* ab) {
     extern __shared__ float shm[];
